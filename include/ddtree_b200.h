@@ -29,6 +29,11 @@
  *                        ancestor bitmasks, for callers that only hold the mask
  *   ddt_lm_head_argmax   the verify forward's lm_head (ddtree.py:467-478) fused with
  *                        sample() at temperature 0 (model/utils.py:28-30)
+ *   ddt_page_tables, ddt_paged_qk_norm_rope, ddt_paged_attn
+ *                        no reference counterpart: a paged K/V cache shared by many requests,
+ *                        where the reference keeps one DynamicCache per request
+ *   ddt_sample           model/utils.py:28-35 sample() at temperature > 0, with top-k, top-p and
+ *                        min-p and the uniforms given by the caller
  *   ddt_sample_chains    mdflash.py:19-40 sample_candidate_chains
  *   ddt_chain_tree       ddtree.py:169-224 build_sampled_candidate_tree
  */
@@ -444,6 +449,98 @@ int ddt_silu_mul(const void* gate_up, int64_t rows, int64_t inter, void* out, vo
  * anc_bits [n_nodes, anc_words]. */
 int ddt_mask_to_bits(const void* mask, int dtype, int64_t n_nodes, int64_t row_stride,
                      uint32_t* anc_bits, int64_t anc_words, void* stream);
+
+/* ---- paged K/V cache --------------------------------------------------------
+ * One pool of pages serves many requests: k_pages / v_pages hold n_pages pages of page_size
+ * rows per KV head, element (page, head, row, d) at page * page_stride + head * head_stride +
+ * row * row_stride + d (elements; the same strides for K and V; both [page, head, row] and
+ * [page, row, head] orders are strides).  page_size is a power of two from 16 to 1024.
+ * block_table i32 [n_requests, max_pages] (row stride table_stride): entry j of request r is the page of its rows
+ * [j * page_size, (j + 1) * page_size).  A slot is page * page_size + row.  Lengths, offsets
+ * and tables live on the device, so a recorded step serves every length.  No counterpart in
+ * the reference, which keeps one contiguous cache per request (ddtree.py:387).
+ *
+ * ddt_page_tables: one step of the tables, from every request's length before (old_lens) and
+ * after (new_lens) it, i32 [n_requests].  Requests that shrink (rejected drafts, or 0 for one
+ * that ended) give pages back: they go on top of the free stack free_pages[0, *free_count),
+ * requests in order, a request's pages in order.  Then requests that grow take theirs from the
+ * top, in the same order.  Outputs: block_table (the taken entries) and free_pages in place;
+ * kv_lens i32 [n_requests] = new_lens; cu_new i32 [n_requests + 1], the exclusive prefix of the
+ * new tokens max(new - old, 0); slot_map / positions i64 [max_tokens]: slot and position of
+ * every new token, requests in order (-1 and 0 after the last one); free_count_out.
+ * All or nothing: with too few free pages, a length that is negative or beyond max_pages pages,
+ * more than max_tokens new tokens or a free stack beyond free_capacity, nothing moves, kv_lens =
+ * old_lens, there are no new tokens and *status gets DDT_STATUS_PAGES.  kv_lens may be old_lens
+ * or new_lens, free_count_out may be free_count (in place).  At most DDT_MAX_PAGED_REQUESTS.
+ * The workspace (ddt_page_tables_workspace_bytes) must be zero-filled before its first use;
+ * every launch leaves it zeroed.
+ *
+ * ddt_paged_qk_norm_rope: like ddt_qk_norm_rope_cache_table with the K / V rows written to
+ * their slots: from the fused projection qkv [n_tokens, q_heads + 2 kv_heads, head_dim] (row
+ * stride qkv_stride elements) q and k get their RMS norm and rotary embedding (rope_table of
+ * ddt_rope_table), q goes to q_out [n_tokens, q_heads, head_dim], k and v to row slot_map[i] of
+ * the pool.  A slot outside the pool (-1: padding) writes no K / V.  Rounded to bf16 once.
+ *
+ * ddt_paged_attn: causal attention of every request's new tokens over its pages.  Request r
+ * owns query rows [cu_new[r], cu_new[r + 1]) of q [n_tokens, q_heads, head_dim] (element
+ * strides), at positions kv_lens[r] - n_r .. kv_lens[r] - 1 (n_r its new tokens, their K / V
+ * already in the pool); each sees the keys up to its own position.  A row that sees no key
+ * (kv_lens[r] < n_r) gives 0.  Rows of q that no request owns are not written.  Rows beyond
+ * kv_lens[r] of a page may hold anything; rows below it must be finite.  max_new bounds n_r
+ * (it picks the kernel).  A request whose lengths are out of range (n_r outside [0, max_new],
+ * rows outside [0, n_tokens], kv_lens[r] outside [0, max_pages * page_size]) is skipped and
+ * *status gets DDT_STATUS_PAGED_RANGE.  head_dim 128, q_heads a multiple of kv_heads, at most
+ * 64 query heads per KV head.
+ * The workspace (ddt_paged_attn_workspace_bytes) must be zero-filled before its first use. */
+#define DDT_MAX_PAGED_REQUESTS 2048
+#define DDT_STATUS_PAGES 16
+#define DDT_STATUS_PAGED_RANGE 32
+size_t ddt_page_tables_workspace_bytes(int64_t n_requests);
+int ddt_page_tables(const int32_t* old_lens, const int32_t* new_lens, int64_t n_requests,
+                    int32_t* block_table, int64_t table_stride, int64_t max_pages,
+                    int64_t page_size, int32_t* free_pages, int64_t free_capacity,
+                    const int32_t* free_count, int32_t* kv_lens, int32_t* cu_new,
+                    int64_t* slot_map, int64_t* positions, int64_t max_tokens,
+                    int32_t* free_count_out, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream);
+int ddt_paged_qk_norm_rope(const void* qkv, int64_t qkv_stride, int64_t n_tokens, int64_t q_heads,
+                           int64_t kv_heads, int64_t head_dim, const void* q_norm_w,
+                           const void* k_norm_w, float eps, const void* rope_table,
+                           const int64_t* slot_map, void* q_out, void* k_pages, void* v_pages,
+                           int64_t n_pages, int64_t page_size, int64_t page_stride,
+                           int64_t head_stride, int64_t row_stride, void* stream);
+size_t ddt_paged_attn_workspace_bytes(int64_t n_tokens, int64_t max_new, int64_t q_heads,
+                                      int64_t kv_heads);
+int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                   const void* k_pages, const void* v_pages, int64_t n_pages, int64_t page_size,
+                   int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                   const int32_t* block_table, int64_t table_stride, int64_t max_pages,
+                   const int32_t* cu_new, const int32_t* kv_lens, int64_t n_requests,
+                   int64_t n_tokens, int64_t max_new, int64_t q_heads, int64_t kv_heads,
+                   int64_t head_dim, float scale, void* out, int64_t o_token_stride,
+                   int64_t o_head_stride, void* workspace, size_t workspace_bytes,
+                   int32_t* status, void* stream);
+
+/* ---- sampling from given uniforms ---------------------------------------------
+ * One token per row of logits [rows, vocab] (DDT_F32 or DDT_BF16, row stride in elements), with
+ * per-row temperature, top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off) and the uniform
+ * u in [0, 1); top_k / top_p / min_p may be NULL (off for all rows).
+ * With z_i = (x_i - max x) / temperature (0 where x_i is the maximum) the weight of token i is
+ * the whole number floor(exp(z_i) * 2^40): sums of weights are exact, so a row's token does not
+ * depend on the launch, the batch or the order of the sums.  Kept are the first tokens by (logit
+ * descending, index ascending): top_k of them; of these the fewest whose weight reaches top_p of
+ * the weight of all of these (at least one); of these the ones with exp(z_i) >= min_p (at most
+ * 1).  tokens[r] (i64) is the first token by index whose running kept weight exceeds floor(u *
+ * total); logprobs[r] (f32, may be NULL) the log of its share of the kept weight.  temperature <
+ * 1e-5 keeps the first token alone.  NaN logits count as -inf; -inf tokens are never drawn; a row
+ * with no other gives token -1 and logprob -inf.  vocab < 2^22.
+ * Replaces sample() at temperature > 0 (model/utils.py:28-35: softmax and torch.multinomial).
+ * The workspace (ddt_sample_workspace_bytes; may be 0) needs no initialisation. */
+size_t ddt_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+               const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int64_t* tokens, float* logprobs, void* workspace,
+               size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,7 @@ DDT_MASK_NONE = 2
 DDT_MAX_BUDGET = 1024
 DDT_MAX_DEPTH = 20
 DDT_MAX_NODES = DDT_MAX_BUDGET + 1
+DDT_MAX_PAGED_REQUESTS = 2048
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int64
@@ -90,6 +91,16 @@ SIGNATURES = {
     "ddt_qk_norm_rope_cache_table_device_past": (_i, [_P, _I, _I, _I, _I, _P, _P, _F, _P, _P, _P,
                                                       _P, _I, _I, _I, _P, _P]),
     "ddt_silu_mul": (_i, [_P, _I, _I, _P, _P]),
+    "ddt_page_tables_workspace_bytes": (_S, [_I]),
+    "ddt_page_tables": (_i, [_P, _P, _I, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P,
+                             _S, _P, _P]),
+    "ddt_paged_qk_norm_rope": (_i, [_P, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _P, _P, _P, _I, _I,
+                                    _I, _I, _I, _P]),
+    "ddt_paged_attn_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "ddt_paged_attn": (_i, [_P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I,
+                            _I, _I, _I, _F, _P, _I, _I, _P, _S, _P, _P]),
+    "ddt_sample_workspace_bytes": (_S, [_I, _I]),
+    "ddt_sample": (_i, [_P, _i, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
 
 

@@ -17,6 +17,7 @@ __all__ = [
     "anc_words_for", "TreeBatch", "topk_tree_batched", "KvBatch", "accept_compact_batched",
     "attention_status", "check_status", "tree_attention_wait_check",
     "sample_chains", "chain_tree", "lm_head_argmax",
+    "PageStep", "page_tables", "paged_qk_norm_rope", "paged_attention", "sample",
 ]
 
 
@@ -113,6 +114,8 @@ STATUS_TIMEOUT = 1      # a bounded wait of a kernel ran out
 STATUS_LAYOUT = 2       # a batched compaction met a head stride it cannot move
 STATUS_PAST_RANGE = 4   # a device-side prefix length was outside [0, planned maximum]
 STATUS_LOG_FULL = 8     # a decode-loop round found its output or length log full
+STATUS_PAGES = 16       # a page-table step was refused (pool exhausted or a bad length)
+STATUS_PAGED_RANGE = 32  # paged attention skipped a request whose lengths are out of range
 
 
 def check_status(status: torch.Tensor, what: str = "ddt_tree_attn") -> None:
@@ -126,7 +129,9 @@ def check_status(status: torch.Tensor, what: str = "ddt_tree_attn") -> None:
         if v & STATUS_TIMEOUT:
             check(_lib.DDT_ERR_TIMEOUT, what)
         why = ("prefix length out of range" if v & STATUS_PAST_RANGE else
-               "decode-loop log full" if v & STATUS_LOG_FULL else "invalid KV layout")
+               "decode-loop log full" if v & STATUS_LOG_FULL else
+               "page-table step refused" if v & STATUS_PAGES else
+               "paged request out of range" if v & STATUS_PAGED_RANGE else "invalid KV layout")
         raise _lib.DDTreeError(f"{what}: device status {v:#x} ({why})")
 
 
@@ -850,3 +855,204 @@ def mask_to_bits(mask_block: torch.Tensor, words: int | None = None) -> torch.Te
           "ddt_mask_to_bits")
     STATS.launches += 1
     return bits
+
+
+# ---- paged K/V cache and sampling ------------------------------------------------------
+@dataclass
+class PageStep:
+    """What a page-table step hands to the kernels of the same step (all on the device)."""
+    kv_lens: torch.Tensor      # i32 [R], the lengths after the step
+    cu_new: torch.Tensor       # i32 [R + 1], exclusive prefix of the new tokens
+    slot_map: torch.Tensor     # i64 [max_tokens], page * page_size + row, -1 past the last token
+    positions: torch.Tensor    # i64 [max_tokens]
+    free_count: torch.Tensor   # i32 [1], pages left on the free stack
+
+    @staticmethod
+    def allocate(device, n_requests: int, max_tokens: int) -> "PageStep":
+        i32 = dict(dtype=torch.int32, device=device)
+        i64 = dict(dtype=torch.int64, device=device)
+        return PageStep(torch.empty(n_requests, **i32), torch.empty(n_requests + 1, **i32),
+                        torch.empty(max_tokens, **i64), torch.empty(max_tokens, **i64),
+                        torch.empty(1, **i32))
+
+
+def _need(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
+
+
+def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+                max_tokens: int, out: PageStep | None = None,
+                status: torch.Tensor | None = None) -> PageStep:
+    """ddt_page_tables: one step of the paged cache's tables in one launch.  old_lens /
+    new_lens i32 [R]: every request's length before and after the step (a shorter one rolls
+    back, 0 releases).  block_table i32 [R, max_pages] and the free stack free_pages i32 [cap] /
+    free_count i32 [1] are updated: block_table and free_pages in place, the count into
+    out.free_count (which may be free_count; out.kv_lens may be old_lens or new_lens).
+    max_tokens bounds the step's new tokens.  A step that does not fit changes nothing and
+    reports itself in the status word (check_status)."""
+    dev = _require_cuda(old_lens, new_lens, block_table, free_pages, free_count)
+    R = old_lens.numel()
+    _need(old_lens, torch.int32, (R,), "old_lens")
+    _need(new_lens, torch.int32, (R,), "new_lens")
+    _need(free_count, torch.int32, (1,), "free_count")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R or \
+            block_table.stride(1) != 1:
+        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise ValueError("free_pages must be a contiguous i32 vector")
+    if out is None:
+        out = PageStep.allocate(dev, R, max_tokens)
+    else:
+        _require_cuda(old_lens, out.kv_lens, out.cu_new, out.slot_map, out.positions,
+                      out.free_count)
+        _need(out.kv_lens, torch.int32, (R,), "out.kv_lens")
+        _need(out.cu_new, torch.int32, (R + 1,), "out.cu_new")
+        _need(out.slot_map, torch.int64, (max_tokens,), "out.slot_map")
+        _need(out.positions, torch.int64, (max_tokens,), "out.positions")
+        _need(out.free_count, torch.int32, (1,), "out.free_count")
+    if status is None:
+        status = attention_status(dev)
+    lib = _lib.load()
+    ws = WORKSPACES.get(dev, "page_tables", lib.ddt_page_tables_workspace_bytes(R))
+    check(lib.ddt_page_tables(
+        old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
+        block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], page_size,
+        free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), out.kv_lens.data_ptr(),
+        out.cu_new.data_ptr(), out.slot_map.data_ptr(), out.positions.data_ptr(), max_tokens,
+        out.free_count.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)),
+        "ddt_page_tables")
+    STATS.launches += 1
+    return out
+
+
+def _pages_view(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """(n_pages, kv_heads, page_size, page stride, head stride, row stride) of a page pool:
+    logical [pages, kv_heads, page_size, 128] bf16 with any strides but the last."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
+            k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        raise ValueError("k_pages / v_pages must be [pages, kv_heads, page_size, head_dim] with "
+                         "the same strides and contiguous rows")
+    if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
+        raise TypeError("paged K/V are bf16")
+    n, h, ps, _ = k_pages.shape
+    sp, sh, sr, _ = k_pages.stride()
+    return n, h, ps, sp, sh, sr
+
+
+def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
+                       rope_table: torch.Tensor, slot_map: torch.Tensor, k_pages: torch.Tensor,
+                       v_pages: torch.Tensor, eps: float = 1e-6,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """ddt_paged_qk_norm_rope: RMS norm and rotary embedding of q and k of the fused projection
+    qkv [T, (q_heads + 2 kv_heads) * 128] (bf16), K / V rows into slot slot_map[i] (i64 [>= T];
+    -1 writes none) of the page pool [pages, kv_heads, page_size, 128].  rope_table i32 [T, 64]
+    (ddt_rope_table).  Returns q [T, q_heads, 128]."""
+    dev = _require_cuda(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages, v_pages)
+    n_pages, hkv, ps, sp, sh, sr = _pages_view(k_pages, v_pages)
+    d = k_pages.shape[3]
+    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or qkv.shape[1] % d:
+        raise ValueError("qkv must be bf16 [tokens, heads * head_dim] with unit stride")
+    T = qkv.shape[0]
+    hq = qkv.shape[1] // d - 2 * hkv
+    if hq <= 0:
+        raise ValueError("qkv holds no query heads beside the pool's KV heads")
+    if q_norm_w.dtype != torch.bfloat16 or k_norm_w.dtype != torch.bfloat16 or \
+            q_norm_w.numel() != d or k_norm_w.numel() != d:
+        raise ValueError("norm weights must be bf16 [head_dim]")
+    _need(rope_table, torch.int32, (T, d // 2), "rope_table")
+    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or slot_map.numel() < T or \
+            not slot_map.is_contiguous():
+        raise ValueError("slot_map must be contiguous i64 with a slot per token")
+    if out is None:
+        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=dev)
+    else:
+        _need(out, torch.bfloat16, (T, hq, d), "out")
+        _require_cuda(qkv, out)
+    check(_lib.load().ddt_paged_qk_norm_rope(
+        qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), T, hq, hkv, d, q_norm_w.data_ptr(),
+        k_norm_w.data_ptr(), eps, rope_table.data_ptr(), slot_map.data_ptr(), out.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, sp, sh, sr, _stream(dev)),
+        "ddt_paged_qk_norm_rope")
+    STATS.launches += 1
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    block_table: torch.Tensor, cu_new: torch.Tensor, kv_lens: torch.Tensor,
+                    max_new: int, scale: float | None = None, out: torch.Tensor | None = None,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """ddt_paged_attn: causal attention of the new tokens q [T, q_heads, 128] (bf16) of R
+    requests over their pages.  cu_new i32 [R + 1] and kv_lens i32 [R] come from page_tables
+    (the new rows' K / V are already in the pool); max_new is the host's bound on the new
+    tokens of one request.  Returns [T, q_heads, 128]; rows that no request owns are not
+    written."""
+    dev = _require_cuda(q, k_pages, v_pages, block_table, cu_new, kv_lens)
+    n_pages, hkv, ps, sp, sh, sr = _pages_view(k_pages, v_pages)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.stride(2) != 1:
+        raise ValueError("q must be bf16 [tokens, q_heads, head_dim] with contiguous rows")
+    T, hq, d = q.shape
+    if d != k_pages.shape[3]:
+        raise ValueError("q and the pages differ in head_dim")
+    R = kv_lens.numel()
+    _need(kv_lens, torch.int32, (R,), "kv_lens")
+    _need(cu_new, torch.int32, (R + 1,), "cu_new")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R or \
+            block_table.stride(1) != 1:
+        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
+    if out is None:
+        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
+        raise ValueError("out must be like q")
+    if status is None:
+        status = attention_status(dev)
+    lib = _lib.load()
+    ws = WORKSPACES.get(dev, "paged_attn", lib.ddt_paged_attn_workspace_bytes(T, max_new, hq, hkv))
+    check(lib.ddt_paged_attn(
+        q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+        sp, sh, sr, block_table.data_ptr(), block_table.stride(0) if R > 1 else block_table.shape[1],
+        block_table.shape[1], cu_new.data_ptr(), kv_lens.data_ptr(), R, T, max_new, hq, hkv, d,
+        d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
+        ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)), "ddt_paged_attn")
+    STATS.launches += 1
+    return out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+           min_p: torch.Tensor | None = None, out: torch.Tensor | None = None,
+           logprobs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """ddt_sample: one token per row of logits [rows, vocab] (f32 or bf16) from the given
+    uniforms u f32 [rows], with per-row temperature f32, top_k i32, top_p f32 and min_p f32
+    (None: off).  Returns (tokens i64 [rows], logprobs f32 [rows]); -1 and -inf for a row
+    without a token to draw."""
+    dev = _require_cuda(logits, u, temperature)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [rows, vocab] with unit stride")
+    rows, vocab = logits.shape
+    _need(u, torch.float32, (rows,), "u")
+    _need(temperature, torch.float32, (rows,), "temperature")
+    for t, dt, name in ((top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
+                        (min_p, torch.float32, "min_p")):
+        if t is not None:
+            _require_cuda(logits, t)
+            _need(t, dt, (rows,), name)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    else:
+        _need(out, torch.int64, (rows,), "out")
+    if logprobs is None:
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    else:
+        _need(logprobs, torch.float32, (rows,), "logprobs")
+    lib = _lib.load()
+    ws = WORKSPACES.get(dev, "sample", lib.ddt_sample_workspace_bytes(rows, vocab))
+    check(lib.ddt_sample(
+        logits.data_ptr(), _dtype_code(logits), rows, vocab, max(logits.stride(0), vocab),
+        u.data_ptr(), temperature.data_ptr(), top_k.data_ptr() if top_k is not None else None,
+        top_p.data_ptr() if top_p is not None else None,
+        min_p.data_ptr() if min_p is not None else None, out.data_ptr(), logprobs.data_ptr(),
+        ws.data_ptr(), ws.numel(), _stream(dev)), "ddt_sample")
+    STATS.launches += 1
+    return out, logprobs
