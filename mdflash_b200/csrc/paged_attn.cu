@@ -5,139 +5,695 @@
 // with the running maximum m and sum l of a one-pass softmax: a new maximum m' rescales what
 // was summed by 2^(m - m').  A row that sees no key gives 0.
 //
-// One CTA per (token, KV head), one warp per key at a time; the heads of the group share the
-// key.
+// Work unit: one KV head and two tiles of 128 query rows, row = (token, query head of the
+// group), token-major, so that the whole group shares every K / V tile of 128 keys.  A group
+// that does not divide 128 leaves the last 128 mod group rows of each tile unused.  Units are
+// distributed by paged_sched.cuh.  Warp roles (12 warps):
+//   warp 0      producer: Q tiles and, page by page, K and V tiles by TMA (128-byte swizzle,
+//               two stages each; the lanes issue a tile's page boxes side by side, the next
+//               tile's page ids are read one tile ahead).  Pages past the request's last one
+//               are read from beyond the pool, where the tensor map fills zeros.
+//   warps 1, 3  MMA issuers of query tile 0 and 1: S = Q K^T into TMEM, O += P V with P read
+//               from TMEM.  They take turns, so the two softmax warpgroups stay half a period
+//               apart.
+//   warp 2      zeroes the V rows of a request's last page that lie past its length: they may
+//               hold anything, and 0 * NaN would reach every row of the tile (K needs no care:
+//               its scores are replaced by the mask).
+//   warps 4-11  softmax, one query row per thread: the S row in one TMEM read, masked maximum,
+//               P = exp2 back to TMEM as bf16 in two halves.  P is rounded to bf16 because the
+//               matrix instruction takes it so; the row sum l is of the unrounded values (adding
+//               the rounded ones instead makes a lone heavy key exact but costs 4.7%: four chunks
+//               of 2048 tokens, 7k keys each on average, 457 against 437 us).  O is rescaled in
+//               TMEM only when the maximum grew by more than 2^8.
+// TMEM columns: S0/P0 [0,128) O0 [128,256) S1/P1 [256,384) O1 [384,512).
+// Every wait is bounded; a timeout sets *status and unwinds the CTA.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "paged_sched.cuh"
 #include "tc.cuh"
 
 namespace ddt {
 namespace paged_attn {
 
-constexpr int kHeadDim = 128;
-constexpr int kMaxGroup = 64;
-constexpr int kWarps = 8;
+constexpr int kBlockM = 128;
+constexpr int kBlockN = 128;
+constexpr int kStages = 2;
+constexpr int kThreads = 384;
+// Register split (setmaxnreg): 384 threads are launched with 168 registers each; warpgroup 0
+// goes down to 64, the softmax warpgroups up to 216: 128 * 64 + 256 * 216 <= 384 * 168.
+constexpr int kRegsLaunch = 168;
+constexpr int kRegsControl = 64;
+constexpr int kRegsSoftmax = 216;
+static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch,
+              "register split exceeds the launch's registers");
+constexpr int kUnitRows = 2 * kBlockM;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr uint64_t kTimeoutNs = 2000000000ull;
+constexpr uint32_t kHalfBytes = kBlockM * 64 * 2;  // one 64-dim half of a 128-row tile
+constexpr uint32_t kTileBytes = 2 * kHalfBytes;    // 32 KB
+constexpr uint32_t kSmemQ = 0;                     // Q0, Q1
+constexpr uint32_t kSmemK = kSmemQ + 2 * kTileBytes;
+constexpr uint32_t kSmemV = kSmemK + kStages * kTileBytes;
+constexpr uint32_t kSmemFirst = kSmemV + kStages * kTileBytes;  // cost prefix of the requests
+inline uint32_t smem_alloc(int64_t n_requests) {
+  return kSmemFirst + static_cast<uint32_t>((n_requests + 1) * sizeof(long long)) + 1024;
+}
+static_assert(kSmemFirst + (DDT_MAX_PAGED_REQUESTS + 1) * 8 + 1024 + 1024 <= 232448,
+              "shared memory");
+constexpr uint32_t kIdescS = tc::idesc_bf16_f32(kBlockM, kBlockN, false, false);
+constexpr uint32_t kIdescPV = tc::idesc_bf16_f32(kBlockM, kHeadDim, false, true);
+constexpr int kStatusTimeout = 1;
+// of every 16 pairs of exponentials, the ones computed by the FMA-pipe polynomial beside MUFU
+constexpr uint32_t kPolyPairs = 0x1249u;
 
-struct Params {
-  const __nv_bfloat16* q;
-  long long q_token_stride, q_head_stride;
-  const __nv_bfloat16* k_pages;
-  const __nv_bfloat16* v_pages;
-  long long page_stride, head_stride, row_stride, n_pages;
-  int page_shift;
-  const int32_t* block_table;
-  long long table_stride, max_keys;
-  const int32_t* cu_new;
-  const int32_t* kv_lens;
-  int n_requests, n_tokens, max_new, group;
-  float scale_log2;
-  __nv_bfloat16* out;
-  long long o_token_stride, o_head_stride;
-  int32_t* status;
+__device__ __forceinline__ uint32_t col_s(int q) { return q ? 256u : 0u; }
+__device__ __forceinline__ uint32_t col_o(int q) { return q ? 384u : 128u; }
+
+struct Bars {
+  uint64_t q_full, q_empty, k_full[kStages], v_full[kStages], k_empty[kStages],
+      v_empty[kStages], v_clean, s_full[2], p_half[2], p_full[2], o_ready[2], mma_done[2];
+  uint32_t issued[2];
+  uint32_t tmem_base;
+  int abort;
 };
 
-// Lengths of request r, or false (and the status bit) where they are out of range.
-__device__ __forceinline__ bool request(const Params& p, int r, int& first, int& n, int& len) {
-  first = p.cu_new[r];
-  const int end = p.cu_new[r + 1];
-  len = p.kv_lens[r];
-  if (first < 0 || end < first || end > p.n_tokens || end - first > p.max_new || len < 0 ||
-      len > p.max_keys) {
-    if (p.status) atomicOr(p.status, DDT_STATUS_PAGED_RANGE);
-    n = 0;
-    return false;
-  }
-  n = end - first;
-  return true;
+__device__ __forceinline__ void raise_abort(Bars& b, int32_t* status) {
+  *reinterpret_cast<volatile int*>(&b.abort) = 1;
+  if (status) atomicOr(status, kStatusTimeout);
 }
 
-constexpr int kHeads = 4;  // heads of the group per pass over the keys
+// 4-D tiled load into this CTA's shared memory, completion counted on `bar`.
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(tc::smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+      "r"(c3)
+      : "memory");
+}
 
-__global__ void __launch_bounds__(kWarps * 32) paged_attn_simple_kernel(const Params p) {
-  const int tok = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // the request that owns this token
-  int lo = 0, hi = p.n_requests - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_new[mid] <= tok) lo = mid;
-    else hi = mid - 1;
+// whether the item's last tile holds rows past the request's length
+__device__ __forceinline__ bool ragged(const Item& it) {
+  return it.nt > 0 && it.len - (it.t0 + it.nt - 1) * kBlockN < kBlockN;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Bars bars;
+  __shared__ long long s_warp[kThreads / 32];
+  __shared__ Piece piece;
+  __shared__ Place places[kThreads / 32];
+  const uint32_t raw = tc::smem_u32(smem_raw);
+  unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile_tok = kBlockM / p.group;  // tokens per query tile
+  long long* s_first = reinterpret_cast<long long*>(smem + kSmemFirst);
+
+  if (tid == 0) {
+    tc::mbar_init(&bars.q_full, 1);
+    tc::mbar_init(&bars.q_empty, 2);  // one commit per MMA issuer
+    tc::mbar_init(&bars.v_clean, 1);
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(&bars.k_full[s], 1);
+      tc::mbar_init(&bars.v_full[s], 1);
+      tc::mbar_init(&bars.k_empty[s], 2);
+      tc::mbar_init(&bars.v_empty[s], 3);  // and warp 2
+    }
+    for (int q = 0; q < 2; ++q) {
+      tc::mbar_init(&bars.s_full[q], 1);
+      tc::mbar_init(&bars.p_half[q], 4);  // one arrive per softmax warp
+      tc::mbar_init(&bars.p_full[q], 4);
+      bars.issued[q] = 0;
+      tc::mbar_init(&bars.o_ready[q], 1);
+      tc::mbar_init(&bars.mma_done[q], 1);
+    }
+    bars.abort = 0;
+    tc::fence_mbar_init();
   }
-  int first, n, len;
-  if (!request(p, lo, first, n, len) || tok < first || tok >= first + n) return;
-  const int keys = max(len - n + (tok - first) + 1, 0);
-  __shared__ float s_m[kWarps][kHeads], s_l[kWarps][kHeads];
-  __shared__ float s_o[kWarps][kHeads][kHeadDim];
-  for (int g0 = 0; g0 < p.group; g0 += kHeads) {
-    float q[kHeads][4], o[kHeads][4], m[kHeads], l[kHeads];
-#pragma unroll
-    for (int g = 0; g < kHeads; ++g) {
-      m[g] = -INFINITY;
-      l[g] = 0.f;
-      uint2 raw = make_uint2(0, 0);
-      if (g0 + g < p.group)
-        raw = *reinterpret_cast<const uint2*>(p.q + tok * p.q_token_stride +
-                                              (h * p.group + g0 + g) * p.q_head_stride + lane * 4);
-      q[g][0] = __uint_as_float(raw.x << 16);
-      q[g][1] = __uint_as_float(raw.x & 0xffff0000u);
-      q[g][2] = __uint_as_float(raw.y << 16);
-      q[g][3] = __uint_as_float(raw.y & 0xffff0000u);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[g][e] = 0.f;
-    }
-    for (int j = warp; j < keys; j += kWarps) {
-      const long long pg = p.block_table[lo * p.table_stride + (j >> p.page_shift)];
-      if (pg < 0 || pg >= p.n_pages) continue;
-      const long long at = pg * p.page_stride + h * p.head_stride +
-                           (j & ((1 << p.page_shift) - 1)) * p.row_stride + lane * 4;
-      const uint2 kr = *reinterpret_cast<const uint2*>(p.k_pages + at);
-      const uint2 vr = *reinterpret_cast<const uint2*>(p.v_pages + at);
-      const float kf[4] = {__uint_as_float(kr.x << 16), __uint_as_float(kr.x & 0xffff0000u),
-                           __uint_as_float(kr.y << 16), __uint_as_float(kr.y & 0xffff0000u)};
-      const float vf[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u),
-                           __uint_as_float(vr.y << 16), __uint_as_float(vr.y & 0xffff0000u)};
-#pragma unroll
-      for (int g = 0; g < kHeads; ++g) {
-        float s = q[g][0] * kf[0] + q[g][1] * kf[1] + q[g][2] * kf[2] + q[g][3] * kf[3];
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(DDT_FULL_MASK, s, w);
-        s *= p.scale_log2;
-        const float mn = fmaxf(m[g], s);
-        const float alpha = mn == -INFINITY ? 1.f : exp2f(m[g] - mn);
-        const float w = mn == -INFINITY ? 0.f : exp2f(s - mn);
-        m[g] = mn;
-        l[g] = l[g] * alpha + w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[g][e] = o[g][e] * alpha + w * vf[e];
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < kHeads; ++g) {
+  if (warp == 1) {
+    tc::tmem_alloc(&bars.tmem_base, kTmemCols);
+    tc::tmem_relinquish();
+  }
+  walk_begin<kBlockN>(p, 2 * tile_tok, s_first, s_warp, piece, places, kThreads / 32);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = bars.tmem_base;
+  volatile int* abort_flag = &bars.abort;
+  const Item& it = places[warp].it;  // the warp's current item
+  auto next = [&] { return walk_next<kBlockN>(p, 2 * tile_tok, s_first, piece, places[warp]); };
+
+  unsigned char* sQ = smem + kSmemQ;
+  unsigned char* sK = smem + kSmemK;
+  unsigned char* sV = smem + kSmemV;
+
+  if (warp < 4) {
+    tc::reg_dealloc<kRegsControl>();
+    if (warp == 0) {
+      // ---------------------------- TMA producer -------------------------------------
       if (lane == 0) {
-        s_m[warp][g] = m[g];
-        s_l[warp][g] = l[g];
+        tc::tma_prefetch_desc(&tm_q);
+        tc::tma_prefetch_desc(&tm_k);
+        tc::tma_prefetch_desc(&tm_v);
       }
-      *reinterpret_cast<float4*>(&s_o[warp][g][lane * 4]) =
-          make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < kHeads * kHeadDim; x += kWarps * 32) {
-      const int g = x / kHeadDim, d = x % kHeadDim;
-      if (g0 + g < p.group) {
-        float M = -INFINITY, L = 0.f, acc = 0.f;
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][g]);
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = s_m[w][g] == -INFINITY ? 0.f : exp2f(s_m[w][g] - M);
-          L += f * s_l[w][g];
-          acc += f * s_o[w][g][d];
+      // lane l issues box l / 2 of a tile, its dims [64 (l & 1), 64 (l & 1) + 64)
+      const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : kBlockN;
+      const int boxes = kBlockN / box_rows;
+      const bool issues = lane < 2 * boxes;
+      const int half = lane & 1, box_row = (lane >> 1) * box_rows;
+      const uint32_t q_bytes = 2u * static_cast<uint32_t>(tile_tok * p.group) * 128u * 2u;
+      int q_loads = 0, issued_k = 0, issued_v = 0, J = 0, n_item = 0;
+      bool ok = true;
+      auto load_q = [&]() {
+        if (lane == 0) tc::mbar_expect_tx(&bars.q_full, q_bytes);
+        __syncwarp();
+        // a query tile past the last row reads zeros
+        if (lane < 4)
+          tc::tma_load_3d(sQ + (lane >> 1) * kTileBytes + half * kHalfBytes, &tm_q, &bars.q_full,
+                          half * 64, it.h * p.group, it.tok0 + (lane >> 1) * tile_tok);
+        ++q_loads;
+      };
+      // page of this lane's box in key tile t, or n_pages (zeros) past the request's pages
+      auto page_id = [&](int t) -> int {
+        const long long key = static_cast<long long>(t) * kBlockN + box_row;
+        int pg = -1;
+        if (issues && key < it.len)
+          pg = p.block_table[it.r * p.table_stride + (key >> p.page_shift)];
+        return pg >= 0 && pg < p.n_pages ? pg : static_cast<int>(p.n_pages);
+      };
+      while (ok && next()) {
+        const int t0 = it.t0, nt = it.nt;
+        if (nt == 0) continue;
+        int pg_next = page_id(t0);
+        if (n_item == 0) load_q();
+        for (int j = 0; j < nt; ++j) {
+          const int jg = J + j;
+          const int st = jg % kStages;
+          const uint32_t ph = ((jg / kStages) - 1) & 1;  // release phase of tile jg - kStages
+          const int pg = pg_next;
+          if (j + 1 < nt) pg_next = page_id(t0 + j + 1);
+          const int row = static_cast<int>(
+              (static_cast<long long>(t0 + j) * kBlockN + box_row) & ((1 << p.page_shift) - 1));
+          if (jg >= kStages &&
+              !(ok = tc::mbar_wait_warp(&bars.k_empty[st], ph, abort_flag, p.timeout_ns)))
+            break;
+          if (lane == 0) tc::mbar_expect_tx(&bars.k_full[st], kTileBytes);
+          __syncwarp();
+          if (issues)
+            tma_load_4d(sK + st * kTileBytes + half * kHalfBytes + box_row * 128, &tm_k,
+                        &bars.k_full[st], half * 64, row, it.h, pg);
+          issued_k = jg + 1;
+          if (jg >= kStages &&
+              !(ok = tc::mbar_wait_warp(&bars.v_empty[st], ph, abort_flag, p.timeout_ns)))
+            break;
+          if (lane == 0) tc::mbar_expect_tx(&bars.v_full[st], kTileBytes);
+          __syncwarp();
+          if (issues)
+            tma_load_4d(sV + st * kTileBytes + half * kHalfBytes + box_row * 128, &tm_v,
+                        &bars.v_full[st], half * 64, row, it.h, pg);
+          issued_v = jg + 1;
+          if (j == 0 && n_item > 0) {
+            // the item's Q replaces the previous item's once both its S MMAs are done; the
+            // first K / V tile of the item is already on its way
+            if (!(ok = tc::mbar_wait_warp(&bars.q_empty, (n_item - 1) & 1, abort_flag,
+                                          p.timeout_ns)))
+              break;
+            load_q();
+          }
         }
-        p.out[tok * p.o_token_stride + (h * p.group + g0 + g) * p.o_head_stride + d] =
-            __float2bfloat16_rn(L > 0.f ? acc / L : 0.f);
+        J += nt;
+        ++n_item;
+      }
+      if (!ok && lane == 0) raise_abort(bars, p.status);
+      __syncwarp();
+      if (*abort_flag) {
+        // let the loads already in flight land before the CTA releases its shared memory
+        if (q_loads > 0) tc::mbar_wait_drain(&bars.q_full, (q_loads - 1) & 1, kTimeoutNs);
+        for (int j = issued_k > kStages ? issued_k - kStages : 0; j < issued_k; ++j)
+          tc::mbar_wait_drain(&bars.k_full[j % kStages], (j / kStages) & 1, kTimeoutNs);
+        for (int j = issued_v > kStages ? issued_v - kStages : 0; j < issued_v; ++j)
+          tc::mbar_wait_drain(&bars.v_full[j % kStages], (j / kStages) & 1, kTimeoutNs);
+      }
+    } else if (warp == 2) {
+      // ---------------------------- V rows past the length -----------------------------
+      int J = 0;
+      bool ok = true;
+      while (ok && next()) {
+        // every tile is waited for and released, so that this warp keeps step with the stages'
+        // phases
+        const int nt = it.nt;
+        const bool tail = ragged(it);
+        for (int j = 0; j < nt; ++j) {
+          const int jg = J + j, st = jg % kStages;
+          if (!(ok = tc::mbar_wait_warp(&bars.v_full[st], (jg / kStages) & 1, abort_flag,
+                                        p.timeout_ns)))
+            break;
+          if (tail && j + 1 == nt) {
+            const int row0 = it.len - (it.t0 + j) * kBlockN;
+            unsigned char* vd = sV + st * kTileBytes;
+            // whole rows of 128 bytes in either half, so the swizzle does not matter
+            for (int b = row0 * 8 + lane; b < kBlockN * 8; b += 32) {
+              *reinterpret_cast<uint4*>(vd + b * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(vd + kHalfBytes + b * 16) = make_uint4(0, 0, 0, 0);
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bars.v_clean);
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&bars.v_empty[st]);
+        }
+        J += it.nt;
+      }
+      if (!ok && lane == 0) raise_abort(bars, p.status);
+    } else {
+      // ---------------------------- MMA issuers, one per query tile ------------------
+      // The whole warp runs the loop and its waits; an elected lane issues.
+      const int q = warp == 1 ? 0 : 1;
+      // descriptor low words of the Q, K and V tiles; every MMA adds a constant to them
+      constexpr uint32_t kDescHi = tc::desc_sw128_hi(1024);
+      const uint32_t a_q = tc::desc_sw128_lo(tc::smem_u32(sQ), 16) + q * (kTileBytes >> 4);
+      const uint32_t k_lo = tc::desc_sw128_lo(tc::smem_u32(sK), 16);
+      const uint32_t v_lo = tc::desc_sw128_lo(tc::smem_u32(sV), kHalfBytes);
+      const uint32_t d_s = tmem + col_s(q), d_o = tmem + col_o(q);
+      volatile uint32_t* my_turns = &bars.issued[q];
+      const volatile uint32_t* other_turns = &bars.issued[q ^ 1];
+      auto issue_s = [&](int jg, uint32_t turn) {
+        const uint32_t b = k_lo + (jg % kStages) * (kTileBytes >> 4);
+        tc::mma_bf16_ss_w<0>(d_s, a_q, b, kDescHi, kIdescS);
+#pragma unroll
+        for (int kk = 1; kk < kHeadDim / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
+          tc::mma_bf16_ss_w<1>(d_s, a_q + off, b + off, kDescHi, kIdescS);
+          if (kk == kHeadDim / 16 - 1) *my_turns = turn;
+        }
+        tc::mma_commit(&bars.s_full[q]);
+      };
+      auto issue_pv = [&](int jg, int j, int half) {
+        const uint32_t b = v_lo + (jg % kStages) * (kTileBytes >> 4);
+#pragma unroll
+        for (int k4 = 0; k4 < kBlockN / 32; ++k4) {
+          const int kk = half * (kBlockN / 32) + k4;
+          tc::mma_bf16_ts_w(d_o, d_s + kk * 8, b + ((kk * 2048) >> 4), kDescHi, kIdescPV,
+                            (j > 0 || kk > 0) ? 1u : 0u);
+        }
+        if (half) tc::mma_commit(&bars.o_ready[q]);
+      };
+      // plain (volatile) turn counters: they order only the issue of the two tiles' MMAs
+      auto wait_turn = [&](uint32_t target) {
+        uint64_t t0 = 0;
+        for (uint32_t n = 0;; ++n) {
+          if (__all_sync(DDT_FULL_MASK, *other_turns >= target)) return true;
+          if ((n & 255u) == 255u) {
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            if (__any_sync(DDT_FULL_MASK, *abort_flag != 0 || now - t0 > p.timeout_ns))
+              return false;
+          }
+        }
+      };
+      bool ok = true;
+      uint32_t base = 0;
+      int J = 0, n_item = 0, n_ragged = 0;
+      while (ok && next()) {
+        if (it.nt == 0) continue;
+        const int nt = it.nt;
+        const bool tail = ragged(it);
+        if (!(ok = tc::mbar_wait_warp(&bars.q_full, n_item & 1, abort_flag, p.timeout_ns))) break;
+        if (!(ok = tc::mbar_wait_warp(&bars.k_full[J % kStages], (J / kStages) & 1, abort_flag,
+                                      p.timeout_ns)))
+          break;
+        if (!(ok = wait_turn(q == 0 ? base : base + 1))) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+          issue_s(J, base + 1);
+          tc::mma_commit(&bars.k_empty[J % kStages]);
+        }
+        __syncwarp();
+        for (int j = 0; j < nt; ++j) {
+          const int jg = J + j;
+          const int st = jg % kStages;
+          const int sn = (jg + 1) % kStages;
+          const bool more = j + 1 < nt;
+          // K / V of the tile landed long before P_q(j): waited first, while the softmax runs
+          if (!(ok = tc::mbar_wait_warp(&bars.v_full[st], (jg / kStages) & 1, abort_flag,
+                                        p.timeout_ns)))
+            break;
+          if (!more && tail &&
+              !(ok = tc::mbar_wait_warp(&bars.v_clean, n_ragged & 1, abort_flag, p.timeout_ns)))
+            break;
+          if (more && !(ok = tc::mbar_wait_warp(&bars.k_full[sn], ((jg + 1) / kStages) & 1,
+                                                abort_flag, p.timeout_ns)))
+            break;
+          if (!(ok = tc::mbar_wait_warp(&bars.p_half[q], jg & 1, abort_flag, p.timeout_ns))) break;
+          if (!(ok = wait_turn(q == 0 ? base + j + 1 : base + j + 2))) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) issue_pv(jg, j, 0);
+          __syncwarp();
+          if (!(ok = tc::mbar_wait_warp(&bars.p_full[q], jg & 1, abort_flag, p.timeout_ns))) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+            issue_pv(jg, j, 1);
+            tc::mma_commit(&bars.v_empty[st]);
+            if (more) {
+              issue_s(jg + 1, base + j + 2);  // reuses S_q / P_q: runs after the P V above
+              tc::mma_commit(&bars.k_empty[sn]);
+            } else {
+              *my_turns = base + j + 2;
+            }
+          }
+          __syncwarp();
+        }
+        // the item's S MMAs are all issued: Q may be replaced once they are done
+        if (ok && tc::elect_one()) tc::mma_commit(&bars.q_empty);
+        __syncwarp();
+        base += nt + 1;
+        J += nt;
+        ++n_item;
+        n_ragged += tail;
+      }
+      if (!ok && lane == 0) raise_abort(bars, p.status);
+      // every MMA and commit of this warp is done before the CTA's barriers and TMEM go
+      if (n_item > 0 || !ok) {
+        if (tc::elect_one()) tc::mma_commit(&bars.mma_done[q]);
+        __syncwarp();
+        tc::mbar_wait_drain(&bars.mma_done[q], 0, kTimeoutNs);
       }
     }
-    __syncthreads();
+  } else {
+    tc::reg_alloc<kRegsSoftmax>();
+    // ---------------------------- softmax warpgroups -------------------------------
+    const int q = (warp - 4) >> 2;  // query tile of this warpgroup (warps 4-7 / 8-11)
+    const int wq = warp & 3;        // TMEM lane quarter a warp may access: warp id % 4
+    const int r = wq * 32 + lane;
+    const uint32_t tl = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    const uint32_t tS = tl + col_s(q);
+    const uint32_t tO = tl + col_o(q);
+    const float sl2 = p.scale_log2;
+    const tc::Exp2Poly exp2_poly;
+    const int row_tok = r / p.group;               // token of this row within its tile
+    const int row_head = r - row_tok * p.group;
+    const bool row_used = row_tok < tile_tok;
+    bool ok = true;
+    int J = 0;
+    while (next()) {
+      const int tok = q * tile_tok + row_tok;  // token of this row within the unit
+      const bool valid = row_used && tok < it.n_tok;
+      // keys this row sees: [0, lim); rows that are not stored see them all
+      const int lim = valid ? it.past + tok + 1 : 0x7fffffff;
+      const int t0 = it.t0, nt = it.nt;
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; ok && j < nt; ++j) {
+        const int jg = J + j;
+        if (!tc::mbar_wait_warp(&bars.s_full[q], jg & 1, abort_flag, p.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const int left = lim - (t0 + j) * kBlockN;  // columns [0, left) are visible
+        const bool masked = __any_sync(DDT_FULL_MASK, left < kBlockN);
+        // the whole S row (128 fp32) comes out of TMEM in one round trip
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, sv[c]);
+        tc::tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= left) sv[c][e] = __float_as_uint(-INFINITY);
+        }
+        // row max of the raw scores: three-input maxima in 8 independent chains
+        float mx8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            mx8[(e >> 1) & 7] = tc::fmax3(mx8[(e >> 1) & 7], __uint_as_float(sv[c][e]),
+                                          __uint_as_float(sv[c][e + 1]));
+        const float mx = tc::fmax3(tc::fmax3(mx8[0], mx8[1], mx8[2]),
+                                   tc::fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+        bool rescale = false;
+        float alpha = 1.f;
+        if (mx > -INFINITY) {
+          const float ms = mx * sl2;
+          if (m_used == -INFINITY) {
+            m_used = ms;
+            l = 0.f;  // what the polynomial lanes made of masked keys
+          } else if (ms > m_used + kRescaleLog2) {
+            alpha = tc::ex2_approx(m_used - ms);
+            m_used = ms;
+            rescale = true;
+          }
+        }
+        if (__any_sync(DDT_FULL_MASK, rescale)) {
+          // O_q is stable once the previous P V MMA of this item completed
+          if (j > 0 &&
+              !tc::mbar_wait_warp(&bars.o_ready[q], (jg - 1) & 1, abort_flag, p.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tc::tmem_ld32(tO + c * 32, o);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tc::tmem_st32(tO + c * 32, o);
+          }
+          l *= alpha;
+        }
+        const float nm = (m_used == -INFINITY) ? 0.f : -m_used;
+        // P = exp2(S * scale - m), packed bf16 into columns [0, 64) of S_q (masked keys hold
+        // -inf and give 0, or 2^-126 on the polynomial lanes)
+        const uint64_t sl2x2 = tc::f2_pack(sl2, sl2), nmx2 = tc::f2_pack(nm, nm);
+        uint64_t ls2[4] = {0ull, 0ull, 0ull, 0ull};
+        // keys [0, 64) first: their P columns are stored and signalled (p_half) while the
+        // second half is computed, so the first four P V MMAs overlap it
+        uint32_t pk[2][32];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const uint64_t x = tc::f2_fma(tc::f2_pack(__uint_as_float(sv[hf * 2 + c][e]),
+                                                        __uint_as_float(sv[hf * 2 + c][e + 1])),
+                                            sl2x2, nmx2);
+              float a, b;
+              if ((kPolyPairs >> (e >> 1)) & 1u) {
+                exp2_poly(x, a, b);
+              } else {
+                float y0, y1;
+                tc::f2_unpack(x, y0, y1);
+                a = tc::ex2_approx(y0);
+                b = tc::ex2_approx(y1);
+              }
+              ls2[(e >> 1) & 3] = tc::f2_add(ls2[(e >> 1) & 3], tc::f2_pack(a, b));
+              pk[hf][c * 16 + e / 2] = tc::pack_bf16x2(a, b);
+            }
+          }
+          if (hf == 0) tc::tmem_st32(tS, pk[0]);
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars.p_half[q]);
+        tc::tmem_st32(tS + 32, pk[1]);
+        float l0, l1, l2, l3;
+        tc::f2_unpack(tc::f2_add(ls2[0], ls2[1]), l0, l1);
+        tc::f2_unpack(tc::f2_add(ls2[2], ls2[3]), l2, l3);
+        l += (l0 + l1) + (l2 + l3);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars.p_full[q]);
+      }
+      if (ok && nt > 0 &&
+          !tc::mbar_wait_warp(&bars.o_ready[q], (J + nt - 1) & 1, abort_flag, p.timeout_ns))
+        ok = false;
+      // warp-uniform: O holds this item's sums
+      const bool have = ok && nt > 0;
+      if (have) tc::tc_fence_after();
+      const bool seen = have && m_used > -INFINITY;  // per row: some key was visible
+      if (it.slot >= 0) {
+        // a part: unnormalised O in fp32, [dim / 4][row][4] so that a warp's rows (consecutive)
+        // store 512 contiguous bytes at a time
+        const int ur = q * kBlockM + r;
+        float* op = p.o_part + static_cast<long long>(it.slot) * kUnitRows * kHeadDim + ur * 4;
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          if (have) {
+            tc::tmem_ld32(tO + c * 32, o);
+            tc::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(op + ((c * 32 + e) / 4) * kUnitRows * 4) =
+                  make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (valid)
+          *reinterpret_cast<float2*>(
+              p.ml_part + (static_cast<long long>(it.slot) * kUnitRows + ur) * 2) =
+              make_float2(seen ? m_used : -INFINITY, seen ? l : 0.f);
+      } else {
+        const float inv = seen && l > 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* orow = p.out + (it.tok0 + tok) * p.o_token_stride +
+                              (it.h * p.group + row_head) * p.o_head_stride;
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          if (have) {
+            tc::tmem_ld32(tO + c * 32, o);
+            tc::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 v;
+              v.x = tc::pack_bf16x2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+              v.y = tc::pack_bf16x2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              v.z = tc::pack_bf16x2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              v.w = tc::pack_bf16x2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(orow + c * 32 + e) = v;
+            }
+          }
+        }
+      }
+      // the O columns are read: the next item's first P V MMA may overwrite them (it waits
+      // for this warpgroup's p_half of that item, which comes after this point)
+      tc::tc_fence_before();
+      J += nt;
+      if (!ok) break;
+    }
+    if (!ok && lane == 0) raise_abort(bars, p.status);
+  }
+  // what the merge kernel needs of a unit that starts in this CTA and ends in another: its
+  // first row, tokens, head and last CTA (at most one such unit: the CTA's last item)
+  if (tid == kThreads - 1)
+    p.parts[blockIdx.x] = (it.slot >= 0 && (it.slot & 1) )
+                              ? make_int4(it.tok0, it.n_tok, it.h, it.last_cta)
+                              : make_int4(0, 0, 0, -1);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmemCols);
   }
 }
+
+// ---- merge of the parts ----------------------------------------------------------------
+// o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over the parts of a unit in CTA order, M the
+// largest m_i.  One warp per (unit, 32 rows, 16 dims): lane = row, so that every load is 512
+// contiguous bytes.
+constexpr int kMergeDims = 16;
+constexpr int kMergeWarps = 8;
+
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const Params p) {
+  const int c0 = blockIdx.x;
+  const int4 part = p.parts[c0];
+  if (part.w < 0) return;
+  const int w = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rows32 = w / (kHeadDim / kMergeDims), d0 = (w % (kHeadDim / kMergeDims)) * kMergeDims;
+  const int ur = rows32 * 32 + lane;
+  const int tile_tok = kBlockM / p.group, r = ur % kBlockM;
+  const int row_tok = r / p.group, tok = (ur / kBlockM) * tile_tok + row_tok;
+  if (row_tok >= tile_tok || tok >= part.y) return;
+  float M = -INFINITY, L = 0.f, acc[kMergeDims];
+#pragma unroll
+  for (int e = 0; e < kMergeDims; ++e) acc[e] = 0.f;
+  for (int c = c0; c <= part.w; ++c) {
+    const long long slot = 2 * c + (c == c0 ? 1 : 0);
+    const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + (slot * kUnitRows + ur) * 2);
+    if (ml.x == -INFINITY) continue;
+    const float* op = p.o_part + slot * kUnitRows * kHeadDim + ur * 4;
+    float4 o[kMergeDims / 4];
+#pragma unroll
+    for (int e = 0; e < kMergeDims / 4; ++e)
+      o[e] = *reinterpret_cast<const float4*>(op + (d0 / 4 + e) * kUnitRows * 4);
+    const float Mn = fmaxf(M, ml.x), a = M == -INFINITY ? 0.f : exp2f(M - Mn),
+                b = exp2f(ml.x - Mn);
+    M = Mn;
+    L = L * a + ml.y * b;
+#pragma unroll
+    for (int e = 0; e < kMergeDims / 4; ++e) {
+      acc[4 * e] = acc[4 * e] * a + o[e].x * b;
+      acc[4 * e + 1] = acc[4 * e + 1] * a + o[e].y * b;
+      acc[4 * e + 2] = acc[4 * e + 2] * a + o[e].z * b;
+      acc[4 * e + 3] = acc[4 * e + 3] * a + o[e].w * b;
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  __nv_bfloat16* orow = p.out + (part.x + tok) * p.o_token_stride +
+                        (part.z * p.group + (r - row_tok * p.group)) * p.o_head_stride + d0;
+#pragma unroll
+  for (int e = 0; e < kMergeDims; e += 8) {
+    uint4 v;
+    v.x = tc::pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+    v.y = tc::pack_bf16x2(acc[e + 2] * inv, acc[e + 3] * inv);
+    v.z = tc::pack_bf16x2(acc[e + 4] * inv, acc[e + 5] * inv);
+    v.w = tc::pack_bf16x2(acc[e + 6] * inv, acc[e + 7] * inv);
+    *reinterpret_cast<uint4*>(orow + e) = v;
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  }
+  return fn;
+}
+
+// bf16 tensor map of `rank` dimensions (the first contiguous; strides in elements of the
+// others), 128-byte swizzle, zero fill out of bounds.
+inline int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+                    const int64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return DDT_ERR_CUDA;
+  cuuint64_t bytes[4];
+  for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, bytes, box, es,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DDT_OK : DDT_ERR_ALIGN;
+}
+
+// Workspace: partial O, partial (m, l), and the record of the unit that starts in each CTA.
+constexpr size_t kPartO = size_t(2) * kMaxCtas * kUnitRows * kHeadDim * sizeof(float);
+constexpr size_t kPartMl = size_t(2) * kMaxCtas * kUnitRows * 2 * sizeof(float);
+constexpr size_t kWorkspace = kPartO + kPartMl + kMaxCtas * sizeof(int4);
 
 }  // namespace paged_attn
 }  // namespace ddt
@@ -150,7 +706,7 @@ extern "C" size_t ddt_paged_attn_workspace_bytes(int64_t n_tokens, int64_t max_n
   (void)max_new;
   (void)q_heads;
   (void)kv_heads;
-  return 0;
+  return paged_attn::kWorkspace;
 }
 
 extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -164,15 +720,14 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
                               void* workspace, size_t workspace_bytes, int32_t* status,
                               void* stream) {
   using namespace paged_attn;
-  (void)workspace;
-  (void)workspace_bytes;
   if (n_requests <= 0 || n_tokens < 0 || max_new < 0 || q_heads <= 0 || kv_heads <= 0 ||
-      q_heads % kv_heads || n_pages <= 0 || max_pages <= 0 || table_stride < max_pages)
+      q_heads % kv_heads || n_pages <= 0 || max_pages <= 0 || table_stride < max_pages ||
+      !(scale >= 0.f))
     return DDT_ERR_INVALID;
   if (head_dim != kHeadDim || q_heads / kv_heads > kMaxGroup) return DDT_ERR_CAPACITY;
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return DDT_ERR_CAPACITY;
-  if (n_requests > DDT_MAX_PAGED_REQUESTS || n_tokens > 0x7fffffff || n_pages > 0x7fffffff ||
-      max_pages * page_size > 0x7fffffff || kv_heads > 65535)
+  if (n_requests > DDT_MAX_PAGED_REQUESTS || n_tokens > 0x7fffffff || n_pages >= 0x7fffffff ||
+      max_pages > 0x7fffffff / page_size || kv_heads > 65535)
     return DDT_ERR_CAPACITY;
   if (n_tokens == 0 || max_new == 0) return DDT_OK;
   if (!q || !k_pages || !v_pages || !block_table || !cu_new || !kv_lens || !out)
@@ -181,32 +736,60 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
       q_token_stride % 8 || q_head_stride % 8 || page_stride % 8 || head_stride % 8 ||
       row_stride % 8 || o_token_stride % 8 || o_head_stride % 8)
     return DDT_ERR_ALIGN;
+  if (!workspace || workspace_bytes < kWorkspace) return DDT_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return DDT_ERR_ALIGN;
+  const int64_t group = q_heads / kv_heads;
+  CUtensorMap tm_q, tm_k, tm_v;
+  {
+    const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
+                                static_cast<cuuint64_t>(n_tokens)};
+    const int64_t strides[2] = {q_head_stride, q_token_stride};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group),
+                               static_cast<cuuint32_t>(kBlockM / group)};
+    int rc = make_map(&tm_q, q, 3, dims, strides, box);
+    if (rc) return rc;
+    const cuuint64_t kdims[4] = {kHeadDim, static_cast<cuuint64_t>(page_size),
+                                 static_cast<cuuint64_t>(kv_heads),
+                                 static_cast<cuuint64_t>(n_pages)};
+    const int64_t kstrides[3] = {row_stride, head_stride, page_stride};
+    const cuuint32_t kbox[4] = {64, static_cast<cuuint32_t>(page_size < kBlockN ? page_size : kBlockN),
+                                1, 1};
+    if ((rc = make_map(&tm_k, k_pages, 4, kdims, kstrides, kbox))) return rc;
+    if ((rc = make_map(&tm_v, v_pages, 4, kdims, kstrides, kbox))) return rc;
+  }
   Params p;
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_token_stride = q_token_stride;
-  p.q_head_stride = q_head_stride;
-  p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
-  p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
-  p.page_stride = page_stride;
-  p.head_stride = head_stride;
-  p.row_stride = row_stride;
-  p.n_pages = n_pages;
-  p.page_shift = __builtin_ctzll(static_cast<unsigned long long>(page_size));
   p.block_table = block_table;
   p.table_stride = table_stride;
   p.max_keys = max_pages * page_size;
+  p.n_pages = n_pages;
+  p.page_shift = __builtin_ctzll(static_cast<unsigned long long>(page_size));
   p.cu_new = cu_new;
   p.kv_lens = kv_lens;
   p.n_requests = static_cast<int>(n_requests);
   p.n_tokens = static_cast<int>(n_tokens);
   p.max_new = static_cast<int>(max_new < n_tokens ? max_new : n_tokens);
-  p.group = static_cast<int>(q_heads / kv_heads);
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.group = static_cast<int>(group);
+  p.kv_heads = static_cast<int>(kv_heads);
+  // a scale of 0 (all keys alike) is taken as one too small to tell them apart: a masked score
+  // of -inf keeps its sign
+  p.scale_log2 = fmaxf(scale * 1.4426950408889634f, 1e-30f);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.o_token_stride = o_token_stride;
   p.o_head_stride = o_head_stride;
+  p.o_part = static_cast<float*>(workspace);
+  p.ml_part = p.o_part + kPartO / sizeof(float);
+  p.parts = reinterpret_cast<int4*>(p.ml_part + kPartMl / sizeof(float));
   p.status = status;
-  paged_attn_simple_kernel<<<dim3(static_cast<unsigned>(n_tokens), static_cast<unsigned>(kv_heads)),
-                             kWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.timeout_ns = kTimeoutNs;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const uint32_t smem = smem_alloc(n_requests);
+  if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return DDT_ERR_CUDA;
+  paged_attn_kernel<<<kMaxCtas, kThreads, smem, st>>>(tm_q, tm_k, tm_v, p);
+  const int rc = launch_status();
+  if (rc) return rc;
+  paged_merge_kernel<<<dim3(kMaxCtas, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
+                       kMergeWarps * 32, 0, st>>>(p);
   return launch_status();
 }

@@ -1,0 +1,209 @@
+// Work distribution of the paged attention kernels, computed by every CTA from the device-side
+// lengths (no plan is built on the host or kept between calls, so one recorded launch serves
+// every length).
+//
+// A unit is (KV head, request, up to kTokens consecutive new tokens of it); it attends to the
+// keys [0, past + its last token + 1) in tiles of kTile keys.  Its cost is its tiles plus kItem
+// (loading Q, filling the pipeline, the epilogue; 2 tiles' worth measured for the tree
+// attention).  The units of all heads, head by head, form one line of W cost positions that is
+// cut into equal pieces, one per CTA; a CTA runs the tiles that lie in its piece.  A unit that
+// crosses a cut is finished in parts: the part that holds the unit's first tile goes to slot
+// 2 c + 1 of its CTA c, every later one to slot 2 c of its CTA; they are consecutive CTAs, and
+// a CTA has at most one of each kind.
+#pragma once
+
+#include "common.cuh"
+
+namespace ddt {
+namespace paged_attn {
+
+constexpr int kHeadDim = 128;
+constexpr int kMaxGroup = 64;
+constexpr int kItem = 2;
+constexpr int kMaxCtas = 148;
+
+struct Params {
+  const int32_t* block_table;
+  long long table_stride, max_keys, n_pages;
+  int page_shift;
+  const int32_t* cu_new;
+  const int32_t* kv_lens;
+  int n_requests, n_tokens, max_new, group, kv_heads;
+  float scale_log2;
+  __nv_bfloat16* out;
+  long long o_token_stride, o_head_stride;
+  float* o_part;   // [2 * CTAs][dim / 4][rows per unit][4]
+  float* ml_part;  // [2 * CTAs][rows per unit][2]
+  int4* parts;     // [CTAs]: a unit that starts in this CTA and is finished by others
+  int32_t* status;
+  unsigned long long timeout_ns;
+};
+
+// First query row, new tokens and key count of request r; no tokens (and the status bit, from
+// one CTA) where they are out of range.
+struct Request {
+  int first, n, len;
+};
+__device__ __forceinline__ Request request(const Params& p, int r) {
+  Request q;
+  q.first = p.cu_new[r];
+  const int end = p.cu_new[r + 1];
+  q.len = p.kv_lens[r];
+  const bool fine = q.first >= 0 && end >= q.first && end <= p.n_tokens &&
+                    end - q.first <= p.max_new && q.len >= 0 && q.len <= p.max_keys;
+  q.n = fine ? end - q.first : 0;
+  if (!fine && p.status && blockIdx.x == 0) atomicOr(p.status, DDT_STATUS_PAGED_RANGE);
+  return q;
+}
+
+struct Item {
+  int h, r;
+  int tok0, n_tok;  // query rows of the unit: [tok0, tok0 + n_tok), all heads of the group
+  int past;         // keys before the unit's first token
+  int len;          // keys of the request
+  int t0, nt;       // key tiles of this piece
+  int slot;         // -1: the unit's only piece
+  int last_cta;     // CTA of the unit's last part (parts only)
+};
+
+// The piece of the line that this CTA runs, and a warp's place in it.  Both live in shared
+// memory: the walk is a few dozen instructions of one lane per item, and its state in registers
+// made the kernel's warps spill.
+struct Piece {
+  long long per_head, total, ctas, x0, x1;
+};
+struct Place {
+  int h, r, j;
+  long long u0;
+  Request q;
+  Item it;
+  int more;
+};
+
+template <int kTile>
+__device__ __forceinline__ int tiles_of(const Request& q, int tok_end) {
+  const int end = q.len - q.n + tok_end;
+  return end > 0 ? (end - 1) / kTile + 1 : 0;
+}
+
+// Costs of the requests for one KV head into s_first [n_requests + 1] (exclusive prefix), this
+// CTA's piece, and the place of its first unit; all threads of the block call it.
+template <int kTile>
+__device__ void walk_begin(const Params& p, int tokens, long long* s_first, long long* s_warp,
+                           Piece& piece, Place* places, int n_places) {
+  const int nthr = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.n_requests + nthr - 1) / nthr;
+  const int r0 = min(tid * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
+  long long sum = 0;
+  for (int r = r0; r < r1; ++r) {
+    const Request q = request(p, r);
+    s_first[r] = sum;
+    for (int t = 0; t < q.n; t += tokens) sum += kItem + tiles_of<kTile>(q, min(t + tokens, q.n));
+  }
+  long long incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(DDT_FULL_MASK, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  long long before = incl - sum;
+  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  for (int r = r0; r < r1; ++r) s_first[r] += before;
+  if (tid == nthr - 1) s_first[p.n_requests] = before + sum;
+  __syncthreads();
+  if (tid < n_places) {
+    Piece c;
+    c.per_head = s_first[p.n_requests];
+    c.total = c.per_head * p.kv_heads;
+    c.ctas = c.total < gridDim.x ? c.total : gridDim.x;
+    c.x0 = c.x1 = 0;
+    Place w;
+    w.h = p.kv_heads;
+    w.r = w.j = w.more = 0;
+    w.u0 = 0;
+    w.it.slot = -1;
+    if (blockIdx.x < c.ctas) {
+      c.x0 = blockIdx.x * c.total / c.ctas;
+      c.x1 = (blockIdx.x + 1) * c.total / c.ctas;
+      w.h = static_cast<int>(c.x0 / c.per_head);
+      const long long at = c.x0 - w.h * c.per_head;
+      int lo = 0, hi = p.n_requests - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_first[mid] <= at) lo = mid;
+        else hi = mid - 1;
+      }
+      w.r = lo;
+      w.q = request(p, lo);
+      long long u = s_first[lo];
+      for (;;) {
+        const int cost = kItem + tiles_of<kTile>(w.q, min((w.j + 1) * tokens, w.q.n));
+        if (u + cost > at) break;
+        u += cost;
+        ++w.j;
+      }
+      w.u0 = w.h * c.per_head + u;
+    }
+    places[tid] = w;
+    if (tid == 0) piece = c;
+  }
+}
+
+// The next item of this warp's walk into w.it (whole warp); false after the last one.
+template <int kTile>
+__device__ __forceinline__ bool walk_next(const Params& p, int tokens, const long long* s_first,
+                                          const Piece& c, Place& w) {
+  __syncwarp();  // the previous item is no longer read
+  if ((threadIdx.x & 31) == 0) {
+    w.more = 0;
+    while (w.h < p.kv_heads && w.u0 < c.x1) {
+      const int tok = w.j * tokens, n_tok = min(tokens, w.q.n - tok);
+      const int tiles = tiles_of<kTile>(w.q, tok + n_tok);
+      const long long b = c.x0 - w.u0 - kItem, e = c.x1 - w.u0 - kItem;
+      const int lo = b <= 0 ? 0 : static_cast<int>(b < tiles ? b : tiles);
+      const int hi = e <= 0 ? 0 : static_cast<int>(e < tiles ? e : tiles);
+      const bool here = hi > lo || (tiles == 0 && w.u0 >= c.x0);
+      if (here) {
+        w.it.h = w.h;
+        w.it.r = w.r;
+        w.it.tok0 = w.q.first + tok;
+        w.it.n_tok = n_tok;
+        w.it.past = w.q.len - w.q.n + tok;
+        w.it.len = w.q.len;
+        w.it.t0 = lo;
+        w.it.nt = hi - lo;
+        w.it.slot = hi - lo == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (lo == 0 ? 1 : 0);
+        // piece c holds position x when c * total < (x + 1) * ctas <= (c + 1) * total; the
+        // unit's last position is in the piece of its last part (a search: a 64-bit division
+        // is a call, and made the whole kernel spill around it)
+        int last = blockIdx.x;
+        if (w.it.slot >= 0)
+          while ((last + 1) * c.total < (w.u0 + kItem + tiles) * c.ctas) ++last;
+        w.it.last_cta = last;
+      }
+      ++w.j;
+      w.u0 += kItem + tiles;
+      if (w.j * tokens >= w.q.n) {
+        w.j = 0;
+        do {
+          if (++w.r == p.n_requests) {
+            w.r = 0;
+            ++w.h;
+          }
+        } while (s_first[w.r] == s_first[w.r + 1]);
+        if (w.h < p.kv_heads && w.u0 < c.x1) w.q = request(p, w.r);
+      }
+      if (here) {
+        w.more = 1;
+        break;
+      }
+    }
+  }
+  __syncwarp();
+  return w.more != 0;
+}
+
+}  // namespace paged_attn
+}  // namespace ddt
