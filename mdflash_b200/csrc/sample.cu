@@ -2,20 +2,20 @@
 //
 // Weights are whole numbers, w_i = floor(exp((x_i - max) / T) * 2^40), so every sum of them is
 // exact and the token does not depend on the order in which a launch adds.  The kept tokens are
-// a prefix of the order (logit descending, index ascending), so they are described by a key
-// (the order-preserving image of a logit) and an index: a token is kept when its key is above
-// the key, or equal and its index at most the index.
+// a prefix of the order (logit descending, index ascending), described by its last token: kept
+// are the logits above `edge`, and the equal ones up to index `last`.
 //
 // A row is shared by a cluster of 1 to 8 CTAs; every warp owns a contiguous range of indices and
 // reads it with 16-byte loads in every pass (the first from HBM, the others from L2):
-//   1. the maximum
-//   2. (top-k, top-p) the boundary key, by three radix steps of 11, 11 and 10 bits: counts and
-//      weights of the tokens that share the digits found so far, per value of the next digit;
-//      the histograms of the cluster's CTAs are added by each of them through distributed
-//      shared memory
-//   3. (a cut inside a run of equal logits) the index of the last one kept
-//   4. the weight of the kept tokens; the warp that holds the target then walks its range
-// Passes exchange one value per CTA through distributed shared memory and one cluster barrier.
+//   1. maximum and minimum
+//   2. for top-k (by counts), then for top-p (by weights, of what top-k keeps): a histogram of
+//      the row over 2048 equal intervals of the logits, added over the cluster through
+//      distributed shared memory; the interval that holds the boundary; a pass that lists its
+//      tokens (a few hundred of 152k where the row looks like a model's); and every listed token
+//      compared with every other, which gives each its exact count and weight before it.  Lists of
+//      more than 1024 tokens (long runs of equal logits) are searched by the bits of the key.
+//   3. the weight of the kept tokens; the warp that holds the target then walks its range
+// CTAs exchange values through distributed shared memory, with one cluster barrier each time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -31,6 +31,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
 constexpr int kOwn = kBins / kThreads;  // bins per thread
+constexpr int kList = 1024;
 constexpr double kLogUnit = 27.725887222397812;  // 40 ln 2
 
 struct Args {
@@ -47,14 +48,28 @@ struct Args {
   int vectors;  // rows start at 16-byte boundaries
 };
 
-// exp of the scaled distance to the maximum: a plain division and CUDA's expf, by which the
-// weight is defined
-__device__ __forceinline__ float scaled(float x, float top, float temp) {
-  return x == top ? 0.f : (x - top) / temp;
-}
+// a / b, correctly rounded, for the many a of one b: with y the correctly rounded reciprocal
+// and q within one unit in the last place, q + (a - q b) y rounds to the quotient (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", IBM J. Res.
+// Dev. 34, 1990), unless b's significand is all ones; the first step brings a y that close.
+// Those b, and ones whose reciprocal is not a normal number, take the plain division.
+struct Divisor {
+  float b, y;
+  bool plain;
+  __device__ explicit Divisor(float d) : b(d), y(1.f / d) {
+    plain = (__float_as_uint(d) & 0x7fffffu) == 0x7fffffu || d > 1e30f;
+  }
+  __device__ __forceinline__ float operator()(float a) const {
+    if (plain) return a / b;
+    float q = a * y;
+    q = __fmaf_rn(__fmaf_rn(-q, b, a), y, q);
+    return __fmaf_rn(__fmaf_rn(-q, b, a), y, q);
+  }
+};
+
 // floor(e * 2^40) = hi * 2^20 + lo for e in [0, 1], hi <= 2^20, lo < 2^20: adding 8 with
 // rounding toward zero leaves multiples of 2^-20 in the low mantissa bits (a conversion to 64
-// bits runs at an eighth of the rate)
+// bits runs at a fraction of the rate)
 __device__ __forceinline__ void limbs(float e, uint32_t& hi, uint32_t& lo) {
   const float t = __fadd_rz(e, 8.f);
   hi = __float_as_uint(t) - 0x41000000u;
@@ -66,23 +81,29 @@ __device__ __forceinline__ unsigned long long whole(float e) {
   return (static_cast<unsigned long long>(hi) << 20) + lo;
 }
 
-// What a CTA shows to the others of its cluster; one field per exchange, so that each needs
-// one cluster barrier only.
+// What a CTA shows to the others of its cluster, and its own scratch.
 struct Shared {
   alignas(16) uint32_t count[kBins], lo[kBins], hi[kBins];  // weight of a bin: hi * 2^32 + lo
+  float list_x[kList];                                      // this CTA's part of a list
+  int list_i[kList];
+  float all_x[kList];  // the cluster's list
+  int all_i[kList];
+  unsigned long long all_w[kList];
   unsigned long long warp_sum[2][kWarps];
-  unsigned long long sum;    // kept weight of the CTA
-  uint32_t top_key;
-  int ties, tie_index;
+  unsigned long long sum;  // kept weight of the CTA
+  uint32_t top_key, low_key;
+  int n_list, ties, tie_index;
   // found by one thread of the CTA for all of its threads
   int bin;
   unsigned long long before_c, before_w, bin_c;
+  float edge;
+  int last;
 };
 
 // Exclusive block scan of (c, w) in thread order; returns the totals too.
 __device__ __forceinline__ void scan2(unsigned long long c, unsigned long long w, Shared& s,
                                       unsigned long long& c_before, unsigned long long& w_before,
-                                      unsigned long long& c_all, unsigned long long& w_all) {
+                                      unsigned long long& w_all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long ci = c, wi = w;
 #pragma unroll
@@ -102,29 +123,30 @@ __device__ __forceinline__ void scan2(unsigned long long c, unsigned long long w
   __syncthreads();
   c_before = ci - c;
   w_before = wi - w;
-  c_all = w_all = 0;
-#pragma unroll 8
+  w_all = 0;
+#pragma unroll 4
   for (int k = 0; k < kWarps; ++k) {
     const unsigned long long a = s.warp_sum[0][k], b = s.warp_sum[1][k];
     if (k < warp) {
       c_before += a;
       w_before += b;
     }
-    c_all += a;
     w_all += b;
   }
 }
 
 template <bool kBF16>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   constexpr int kVec = kBF16 ? 8 : 4;  // elements per 16-byte load
   constexpr int kStep = 32 * kVec;
-  __shared__ Shared s;
+  extern __shared__ unsigned char smem_raw[];
+  Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int V = a.vocab;
   const char* x = static_cast<const char*>(a.logits) + row * a.row_stride * (kBF16 ? 2 : 4);
+  auto peer = [&](int r) { return cluster.map_shared_rank(&s, r); };
 
   // this warp's range of indices
   const int per_warp =
@@ -133,7 +155,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
                        static_cast<long long>(V));
   const int seg1 = min(seg0 + per_warp, V);
 
-  // the kVec elements from index i on (-inf past the end; NaN as -inf)
+  // the kVec elements from index i on (NaN past the end: like every NaN they are below all,
+  // equal to none and of weight 0)
+  bool inf_top = false;  // +inf takes all of the weight: the row is then read as 0 and -inf
   auto load = [&](int i, float (&v)[kVec]) {
     if (a.vectors && i + kVec <= seg1) {
       const uint4 r = *reinterpret_cast<const uint4*>(x + static_cast<long long>(i) * (kBF16 ? 2 : 4));
@@ -148,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     } else {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        v[e] = -INFINITY;
+        v[e] = __uint_as_float(0x7fffffffu);
         if (i + e < seg1) {
           if constexpr (kBF16)
             v[e] = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(x)[i + e]);
@@ -157,27 +181,50 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
       }
     }
+    if (inf_top) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) v[e] = isnan(v[e]) ? -INFINITY : v[e];
+      for (int e = 0; e < kVec; ++e) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
+    }
+  };
+  // f(index, value) over this warp's range
+  auto each = [&](auto f) {
+#pragma unroll 2
+    for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
+      float v[kVec];
+      load(i, v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f(i + e, v[e]);
+    }
   };
 
-  // ---- 1. maximum ----------------------------------------------------------------------
-  float mx = -INFINITY;
+  // ---- 1. maximum and minimum ------------------------------------------------------------
+  float mx = -INFINITY, mn = INFINITY;
 #pragma unroll 4
   for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
     float v[kVec];
     load(i, v);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) mx = fmaxf(mx, v[e]);
+    for (int e = 0; e < kVec; ++e) {
+      mx = fmaxf(mx, v[e]);
+      mn = fminf(mn, v[e]);
+    }
   }
   uint32_t top_key = __reduce_max_sync(DDT_FULL_MASK, f32_key(mx));
-  if (tid == 0) s.top_key = 0;
+  uint32_t low_key = __reduce_min_sync(DDT_FULL_MASK, f32_key(mn));
+  if (tid == 0) {
+    s.top_key = 0;
+    s.low_key = ~0u;
+    s.tie_index = V;
+  }
   __syncthreads();
-  if (lane == 0) atomicMax(&s.top_key, top_key);
+  if (lane == 0) {
+    atomicMax(&s.top_key, top_key);
+    atomicMin(&s.low_key, low_key);
+  }
   cluster.sync();
-  top_key = __reduce_max_sync(DDT_FULL_MASK,
-                              lane < ranks ? cluster.map_shared_rank(&s, lane)->top_key : 0u);
-  const float top = key_f32(top_key);
+  top_key = __reduce_max_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->top_key : 0u);
+  low_key = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->low_key : ~0u);
+  float top = key_f32(top_key);
   if (top == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -186,169 +233,219 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     cluster.sync();
     return;
   }
+  if (top == INFINITY) {
+    inf_top = true;
+    top = 0.f;
+    low_key = f32_key(-INFINITY);
+  }
 
   const float temp_in = a.temperature[row];
   const bool greedy = !(temp_in >= 1e-5f);
   const float temp = greedy ? 1.f : temp_in;
+  const float p_in = a.top_p && !greedy ? a.top_p[row] : 1.f;
   const int k_in = a.top_k ? a.top_k[row] : 0;
-  const int k = greedy ? 1 : (k_in > 0 && k_in < V ? k_in : V);
-  const double p = a.top_p && !greedy ? static_cast<double>(a.top_p[row]) : 1.0;
+  const int k = greedy || p_in <= 0.f ? 1 : (k_in > 0 && k_in < V ? k_in : V);
+  const double p = k > 1 ? static_cast<double>(p_in) : 1.0;
   const float min_p = a.min_p && !greedy ? fminf(a.min_p[row], 1.f) : 0.f;
-  // logits this far below the maximum have weight 0: exp(-28) * 2^40 < 1
-  const float floor_x = -28.f * temp;
-  auto weight = [&](float v) {
-    return v - top < floor_x ? 0ull : whole(expf(scaled(v, top, temp)));
-  };
+  const Divisor by_temp(temp);
+  // exp of the scaled distance to the maximum, by CUDA's expf; -200 stands for all that is
+  // far below a weight of 1 and for the NaN of -inf and NaN logits
+  auto scaled = [&](float v) { return fmaxf(by_temp(v - top), -200.f); };
+  auto weight = [&](float v) { return whole(expf(scaled(v))); };
 
-  // ---- 2. boundary key: kept are the keys above `key` and the first `ties` equal to it ----
-  uint32_t key = 0;
-  unsigned long long ties = ~0ull;   // of the `n_ties` tokens with this key
-  unsigned long long n_ties = 0;
-  // One search: the key of token number `want` (counts), or of the last token whose weight
-  // before it is below `reach` (weights).  Of the keys equal to k_key only k_ties count.
-  // Leaves the count / weight of the tokens above the key.
-  auto search = [&](bool by_weight, bool weigh, unsigned long long want, double reach, double frac,
-                    bool bounded, uint32_t k_key, unsigned long long k_ties,
-                    unsigned long long& above_w) {
+  // ---- 2. what top-k and top-p keep -----------------------------------------------------------
+  float edge = -INFINITY;
+  int last = V;
+  auto kept = [&](int i, float v) { return v > edge || (v == edge && i <= last); };
+  // interval of a logit: equal intervals from the maximum down to the minimum, or to where
+  // weights end (the last interval takes the rest)
+  const float span = fminf(top - key_f32(low_key), 28.f * temp);
+  const float per_unit = span > 0.f ? (kBins - 1) / span : 0.f;
+  auto bin_of = [&](float v) {
+    return min(__float2int_rz(__fmul_rn(__fsub_rn(top, v), per_unit)), kBins - 1);
+  };
+  // Histogram of the kept tokens by `bin` (those with a bin >= 0), added over the cluster; then
+  // the bin that holds the boundary: by weight the last one whose weight before it is below
+  // `reach`, else the one that holds token number `want`.  s.bin, s.before_c, s.before_w, s.bin_c.
+  double reach = 0.0;
+  auto boundary = [&](bool by_weight, bool count, bool ascending, unsigned long long want,
+                      unsigned long long above_c, unsigned long long above_w, bool set_reach,
+                      auto bin) {
+    for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
+    __syncthreads();
+    each([&](int i, float v) {
+      const int b = kept(i, v) ? bin(v) : -1;
+      if (b >= 0) {
+        if (by_weight) {
+          const unsigned long long w = weight(v);
+          if (w) {
+            const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&s.lo[b], wl);
+            const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+            if (wh) atomicAdd(&s.hi[b], wh);
+          }
+        }
+        if (count) atomicAdd(&s.count[b], 1u);
+      }
+    });
+    if (tid == 0) s.bin = -1;
+    cluster.sync();
+    // thread t owns kOwn bins, in the order of the tokens
+    unsigned long long c[kOwn] = {}, w[kOwn] = {}, c_sum = 0, w_sum = 0;
+    const int b0 = (ascending ? tid : kThreads - 1 - tid) * kOwn;
+    for (int r = 0; r < ranks; ++r) {
+      const Shared* o = peer(r);
+      if (count) {
+        const uint4 oc = *reinterpret_cast<const uint4*>(&o->count[b0]);
+        c[0] += oc.x, c[1] += oc.y, c[2] += oc.z, c[3] += oc.w;
+      }
+      if (by_weight) {
+        const uint4 ol = *reinterpret_cast<const uint4*>(&o->lo[b0]),
+                    oh = *reinterpret_cast<const uint4*>(&o->hi[b0]);
+        w[0] += (static_cast<unsigned long long>(oh.x) << 32) + ol.x;
+        w[1] += (static_cast<unsigned long long>(oh.y) << 32) + ol.y;
+        w[2] += (static_cast<unsigned long long>(oh.z) << 32) + ol.z;
+        w[3] += (static_cast<unsigned long long>(oh.w) << 32) + ol.w;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      c_sum += c[h];
+      w_sum += w[h];
+    }
+    unsigned long long c0, w0, w_all;
+    scan2(c_sum, w_sum, s, c0, w0, w_all);
+    if (set_reach) reach = p * static_cast<double>(w_all);
+    c0 += above_c;
+    w0 += above_w;
+#pragma unroll
+    for (int g = 0; g < kOwn; ++g) {
+      const int h = ascending ? g : kOwn - 1 - g;
+      const bool here = by_weight ? static_cast<double>(w0) < reach &&
+                                        !(static_cast<double>(w0 + w[h]) < reach)
+                                  : c0 < want && want <= c0 + c[h];
+      if (here) {
+        s.bin = b0 + h;
+        s.before_c = c0;
+        s.before_w = w0;
+        s.bin_c = c[h];
+      }
+      c0 += c[h];
+      w0 += w[h];
+    }
+    __syncthreads();
+  };
+  // Moves (edge, last) to token number `want` of the kept ones, or to the last of them whose
+  // weight before it is below p times the weight of all.
+  auto cut = [&](bool by_weight, unsigned long long want) {
+    if (tid == 0) s.n_list = 0;
+    boundary(by_weight, !by_weight, true, want, 0, 0, by_weight, bin_of);
+    const int bin = s.bin;
+    if (bin < 0) {  // fewer tokens than `want` (NaN is none): all stay, in every CTA alike
+      cluster.sync();  // the histograms are read
+      return;
+    }
+    const unsigned long long above_c = s.before_c, above_w = s.before_w;
+    each([&](int i, float v) {
+      if (kept(i, v) && bin_of(v) == bin) {
+        const int at = atomicAdd(&s.n_list, 1);
+        if (at < kList) {
+          s.list_x[at] = v;
+          s.list_i[at] = i;
+        }
+      }
+    });
+    cluster.sync();
+    int first = lane < ranks ? peer(lane)->n_list : 0;
+    const int n = __reduce_add_sync(DDT_FULL_MASK, first);
+    if (n <= kList) {
+      // every CTA takes the whole list and finds the boundary by itself
+      for (int r = 0, at = 0; r < ranks; ++r) {
+        const Shared* o = peer(r);
+        const int m = __shfl_sync(DDT_FULL_MASK, first, r);
+        for (int j = tid; j < m; j += kThreads) {
+          const float v = o->list_x[j];
+          s.all_x[at + j] = v;
+          s.all_i[at + j] = o->list_i[j];
+          s.all_w[at + j] = by_weight ? weight(v) : 0ull;
+        }
+        at += m;
+      }
+      __syncthreads();
+      int kept_here = 0, order[kList / kThreads] = {};
+#pragma unroll
+      for (int h = 0; h < kList / kThreads; ++h) {
+        const int j = tid + h * kThreads;
+        order[h] = -1;
+        if (j < n) {
+          const float v = s.all_x[j];
+          const int i = s.all_i[j];
+          unsigned long long c = 0, w = 0;
+          for (int o = 0; o < n; ++o) {
+            const float vo = s.all_x[o];
+            if (vo > v || (vo == v && s.all_i[o] < i)) {
+              ++c;
+              w += s.all_w[o];
+            }
+          }
+          if (by_weight ? static_cast<double>(above_w + w) < reach : above_c + c < want) {
+            ++kept_here;
+            order[h] = static_cast<int>(c);
+          }
+        }
+      }
+      kept_here = __reduce_add_sync(DDT_FULL_MASK, kept_here);
+      if (lane == 0) s.warp_sum[0][warp] = kept_here;
+      __syncthreads();
+      int m = 0;
+      for (int w = 0; w < kWarps; ++w) m += static_cast<int>(s.warp_sum[0][w]);
+#pragma unroll
+      for (int h = 0; h < kList / kThreads; ++h)
+        if (order[h] == m - 1) {
+          s.edge = s.all_x[tid + h * kThreads];
+          s.last = s.all_i[tid + h * kThreads];
+        }
+      cluster.sync();  // the lists are read; (edge, last) is there
+      edge = s.edge;
+      last = s.last;
+      return;
+    }
+    // a long list: three steps over the bits of the key, from the top
+    cluster.sync();
     uint32_t prefix = 0;
-    unsigned long long above_c = 0;
-    above_w = 0;
+    unsigned long long c_above = 0, w_above = 0, n_ties = 0;
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
       const int known = level == 0 ? 32 : level == 1 ? 21 : 10;  // key >> known == prefix
       const uint32_t mask = level == 2 ? 1023u : 2047u;
-      for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
-      __syncthreads();
-#pragma unroll 2
-      for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
-        float v[kVec];
-        load(i, v);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const uint32_t kk = f32_key(v[e]);
-          if (i + e < seg1 && (level == 0 || (kk >> known) == prefix) &&
-              (!bounded || kk > k_key)) {
-            const uint32_t b = (kk >> shift) & mask;
-            if (weigh) {
-              const unsigned long long w = weight(v[e]);
-              if (w) {
-                const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&s.lo[b], wl);
-                const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
-                if (wh) atomicAdd(&s.hi[b], wh);
-              }
-            }
-            if (!by_weight || level == 2) atomicAdd(&s.count[b], 1u);
-          }
-        }
-      }
-      cluster.sync();
-      // bins in descending order, kOwn per thread
-      unsigned long long c[kOwn] = {}, w[kOwn] = {}, c_sum = 0, w_sum = 0;
-      const int b0 = kBins - (tid + 1) * kOwn;  // its lowest bin
-      for (int r = 0; r < ranks; ++r) {
-        const Shared* o = cluster.map_shared_rank(&s, r);
-        const uint4 oc = *reinterpret_cast<const uint4*>(&o->count[b0]);
-        c[0] += oc.w, c[1] += oc.z, c[2] += oc.y, c[3] += oc.x;
-        if (weigh) {
-          const uint4 ol = *reinterpret_cast<const uint4*>(&o->lo[b0]),
-                      oh = *reinterpret_cast<const uint4*>(&o->hi[b0]);
-          w[0] += (static_cast<unsigned long long>(oh.w) << 32) + ol.w;
-          w[1] += (static_cast<unsigned long long>(oh.z) << 32) + ol.z;
-          w[2] += (static_cast<unsigned long long>(oh.y) << 32) + ol.y;
-          w[3] += (static_cast<unsigned long long>(oh.x) << 32) + ol.x;
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < kOwn; ++h) {
-        if (bounded && (level == 0 || (k_key >> known) == prefix) &&
-            ((k_key >> shift) & mask) == b0 + kOwn - 1 - h) {
-          c[h] += k_ties;
-          w[h] += k_ties * weight(key_f32(k_key));
-        }
-        c_sum += c[h];
-        w_sum += w[h];
-      }
-      unsigned long long cb, wb, call, wall;
-      scan2(c_sum, w_sum, s, cb, wb, call, wall);
-      if (level == 0 && by_weight) reach = frac * static_cast<double>(wall);
-      if (tid == 0) s.bin = -1;
-      __syncthreads();
-      unsigned long long c0 = above_c + cb, w0 = above_w + wb;
-#pragma unroll
-      for (int h = 0; h < kOwn; ++h) {
-        // the bin that holds the boundary: it starts before it and ends at or past it
-        const bool here = by_weight
-                              ? static_cast<double>(w0) < reach && !(static_cast<double>(w0 + w[h]) < reach)
-                              : c0 < want && want <= c0 + c[h];
-        if (here) {
-          s.bin = b0 + kOwn - 1 - h;
-          s.before_c = c0;
-          s.before_w = w0;
-          s.bin_c = c[h];
-        }
-        c0 += c[h];
-        w0 += w[h];
-      }
-      __syncthreads();
-      // no bin: reach is 0 or less, and the first token alone is kept
-      const uint32_t digit = s.bin < 0 ? (top_key >> shift) & mask : static_cast<uint32_t>(s.bin);
-      if (s.bin >= 0) {
-        above_c = s.before_c;
-        above_w = s.before_w;
-        n_ties = s.bin_c;
-      }
-      prefix = level == 0 ? digit : (prefix << (level == 1 ? 11 : 10)) | digit;
+      boundary(by_weight, !by_weight || level == 2, false, want, c_above, w_above, false,
+               [&](float v) {
+                 const uint32_t key = f32_key(v);
+                 return level == 0 || (key >> known) == prefix ? static_cast<int>((key >> shift) & mask)
+                                                               : -1;
+               });
+      c_above = s.before_c;
+      w_above = s.before_w;
+      n_ties = s.bin_c;
+      prefix = level == 0 ? s.bin : (prefix << (level == 1 ? 11 : 10)) | s.bin;
       cluster.sync();  // the histograms are read
     }
-    key = prefix;
-    ties = by_weight ? 0 : want - above_c;
+    const float value = key_f32(prefix);
+    // how many of the tokens with this logit stay
+    unsigned long long ties = want - c_above;
     if (by_weight) {
-      // of the tokens with this key the first ones whose weight before them is below the reach
-      const unsigned long long each = weight(key_f32(key));
-      unsigned long long a0 = 0, a1 = each ? n_ties : 0;
+      const unsigned long long one = weight(value);
+      unsigned long long a0 = 0, a1 = n_ties;
       while (a0 < a1) {
         const unsigned long long mid = a0 + (a1 - a0) / 2;
-        if (static_cast<double>(above_w + mid * each) < reach) a0 = mid + 1;
+        if (static_cast<double>(w_above + mid * one) < reach) a0 = mid + 1;
         else a1 = mid;
       }
       ties = a0;
-      if (reach <= 0.0) {
-        key = top_key;
-        ties = 1;
-        n_ties = V;
-      }
     }
-  };
-  if (k == 1) {
-    key = top_key;
-    ties = 1;
-    n_ties = V;
-  } else if (k < V || p < 1.0) {
-    unsigned long long above_w = 0;
-    if (k < V) search(false, false, k, 0.0, 0.0, false, 0, 0, above_w);
-    if (p < 1.0) {
-      const uint32_t k_key = key;
-      const unsigned long long k_ties = ties, k_all = n_ties;
-      search(true, true, 0, 0.0, p, k < V, k_key, k_ties, above_w);
-      // the run of equal logits at the top-k boundary is longer than what top-k keeps of it
-      if (k < V && key == k_key) n_ties = k_all;
-    }
-  }
-
-  // ---- 3. index of the last kept token of the boundary key ---------------------------------
-  int last = V;
-  const float edge = key_f32(key);
-  const bool bounded = ties != ~0ull;
-  if (bounded && ties < n_ties) {
+    // and the index of the last of them
     int mine = 0;
-    for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
-      float v[kVec];
-      load(i, v);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) mine += i + e < seg1 && v[e] == edge;
-    }
+    each([&](int i, float v) { mine += v == value && kept(i, v); });
     mine = __reduce_add_sync(DDT_FULL_MASK, mine);
-    __syncthreads();
     if (lane == 0) s.warp_sum[0][warp] = mine;
     if (tid == 0) s.tie_index = V;
     __syncthreads();
@@ -359,55 +456,74 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     }
     if (tid == 0) s.ties = static_cast<int>(all);
     cluster.sync();
-    before += __reduce_add_sync(DDT_FULL_MASK,
-                                lane < rank ? cluster.map_shared_rank(&s, lane)->ties : 0);
-    const long long want = static_cast<long long>(ties) - before;  // of this warp's ties
-    if (want >= 1 && want <= mine) {
-      long long left = want;
+    before += __reduce_add_sync(DDT_FULL_MASK, lane < rank ? peer(lane)->ties : 0);
+    long long left = static_cast<long long>(ties) - before;  // of this warp's
+    if (left >= 1 && left <= mine) {
       for (int i0 = seg0; i0 < seg1; i0 += kStep) {
         const int i = i0 + lane * kVec;
         float v[kVec];
         load(i, v);
-        int n = 0;
+        int m = 0;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) n += i + e < seg1 && v[e] == edge;
-        int incl = n;
+        for (int e = 0; e < kVec; ++e) m += v[e] == value && kept(i + e, v[e]);
+        int incl = m;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int y = __shfl_up_sync(DDT_FULL_MASK, incl, o);
           if (lane >= o) incl += y;
         }
-        const int all_n = __shfl_sync(DDT_FULL_MASK, incl, 31);
-        if (left <= all_n) {
-          int at = incl - n;
+        const int step = __shfl_sync(DDT_FULL_MASK, incl, 31);
+        if (left <= step) {
+          int at = incl - m;
 #pragma unroll
           for (int e = 0; e < kVec; ++e)
-            if (i + e < seg1 && v[e] == edge && ++at == left) s.tie_index = i + e;
+            if (v[e] == value && kept(i + e, v[e]) && ++at == left) s.tie_index = i + e;
           break;
         }
-        left -= all_n;
+        left -= step;
       }
     }
     cluster.sync();
-    last = __reduce_min_sync(DDT_FULL_MASK,
-                             lane < ranks ? cluster.map_shared_rank(&s, lane)->tie_index : V);
+    last = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
+    edge = value;
+    cluster.sync();  // before the next search writes again
+  };
+  if (k == 1) {
+    // the first of the largest
+    int first = V;
+    each([&](int i, float v) { first = v == top ? min(first, i) : first; });
+    first = __reduce_min_sync(DDT_FULL_MASK, first);
+    if (lane == 0) atomicMin(&s.tie_index, first);
+    cluster.sync();
+    edge = top;
+    last = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
+  } else {
+    if (k < V) cut(false, k);
+    if (p < 1.0) cut(true, 0);
   }
 
-  // ---- 4. kept weight, target, token -------------------------------------------------------
-  auto kept = [&](float v, int i) { return !bounded || v > edge || (v == edge && i <= last); };
-  auto kept_weight = [&](float v, int i) -> unsigned long long {
-    if (v - top < floor_x || !kept(v, i)) return 0ull;
-    const float e = expf(scaled(v, top, temp));
-    return e >= min_p ? whole(e) : 0ull;
+  // ---- 3. kept weight, target, token ---------------------------------------------------------
+  auto kept_limbs = [&](int i, float v, uint32_t& hi, uint32_t& lo) {
+    hi = lo = 0;
+    if (kept(i, v)) {
+      const float e = expf(scaled(v));
+      if (e >= min_p) limbs(e, hi, lo);
+    }
   };
   unsigned long long mine = 0;
 #pragma unroll 2
   for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
     float v[kVec];
     load(i, v);
-    // (past the end v is -inf, of weight 0)
+    uint32_t hi = 0, lo = 0;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) mine += kept_weight(v[e], i + e);
+    for (int e = 0; e < kVec; ++e) {
+      uint32_t h, l;
+      kept_limbs(i + e, v[e], h, l);
+      hi += h;
+      lo += l;
+    }
+    mine += (static_cast<unsigned long long>(hi) << 20) + lo;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(DDT_FULL_MASK, mine, o);
@@ -421,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
   }
   if (tid == 0) s.sum = all;
   cluster.sync();
-  unsigned long long total = lane < ranks ? cluster.map_shared_rank(&s, lane)->sum : 0ull;
+  unsigned long long total = lane < ranks ? peer(lane)->sum : 0ull;
   unsigned long long earlier = lane < rank ? total : 0ull;
 #pragma unroll
   for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
@@ -441,7 +557,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
       load(i, v);
       unsigned long long w[kVec], n = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) n += w[e] = kept_weight(v[e], i + e);
+      for (int e = 0; e < kVec; ++e) {
+        uint32_t h, l;
+        kept_limbs(i + e, v[e], h, l);
+        n += w[e] = (static_cast<unsigned long long>(h) << 20) + l;
+      }
       unsigned long long incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -464,9 +584,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
           }
           a.tokens[row] = pick;
           if (a.logprobs)
-            a.logprobs[row] =
-                static_cast<float>(static_cast<double>(scaled(value, top, temp)) -
-                                   (log(static_cast<double>(total)) - kLogUnit));
+            a.logprobs[row] = static_cast<float>(static_cast<double>(scaled(value)) -
+                                                 (log(static_cast<double>(total)) - kLogUnit));
         }
         break;
       }
@@ -503,15 +622,20 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   if (!aligned(logits, size)) return DDT_ERR_ALIGN;
   sample::Args a{logits, static_cast<int>(vocab), row_stride, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs, aligned(logits, 16) && (row_stride * size) % 16 == 0};
-  // as many CTAs per row as keep the rows in one wave (two CTAs per SM), and no
-  // more than leave each warp one load
+  // as many CTAs per row as keep the rows in one wave (two CTAs per SM), and no more than
+  // leave each warp one load
   int ranks = 1;
   while (ranks < sample::kMaxCluster && rows * ranks * 2 <= 2 * 148 &&
          vocab > ranks * sample::kThreads * (16 / size))
     ranks *= 2;
+  auto kernel = dtype == DDT_BF16 ? sample::sample_kernel<true> : sample::sample_kernel<false>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           sizeof(sample::Shared)) != cudaSuccess)
+    return DDT_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
   cfg.blockDim = dim3(sample::kThreads);
+  cfg.dynamicSmemBytes = sizeof(sample::Shared);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -519,9 +643,7 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = dtype == DDT_BF16 ? cudaLaunchKernelEx(&cfg, sample::sample_kernel<true>, a)
-                                          : cudaLaunchKernelEx(&cfg, sample::sample_kernel<false>, a);
-  if (e != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
     cudaGetLastError();
     return DDT_ERR_CUDA;
   }
