@@ -14,7 +14,8 @@
 //      tokens (a few hundred of 152k where the row looks like a model's); and every listed token
 //      compared with every other, which gives each its exact count and weight before it.  Lists of
 //      more than 1024 tokens (long runs of equal logits) are searched by the bits of the key.
-//   3. the weight of the kept tokens; the warp that holds the target then walks its range
+//   3. the weight of the kept tokens; the warps of the CTA that holds the target share the
+//      range of the warp that holds it, until that is one load per lane
 // CTAs exchange values through distributed shared memory, with one cluster barrier each time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -97,7 +98,7 @@ struct Shared {
   int bin;
   unsigned long long before_c, before_w, bin_c;
   float edge;
-  int last;
+  int last, range0, range1;
 };
 
 // Exclusive block scan of (c, w) in thread order; returns the totals too.
@@ -139,6 +140,7 @@ template <bool kBF16>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   constexpr int kVec = kBF16 ? 8 : 4;  // elements per 16-byte load
   constexpr int kStep = 32 * kVec;
+  constexpr int kBatch = 4;
   extern __shared__ unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -155,60 +157,80 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
                        static_cast<long long>(V));
   const int seg1 = min(seg0 + per_warp, V);
 
-  // the kVec elements from index i on (NaN past the end: like every NaN they are below all,
-  // equal to none and of weight 0)
   bool inf_top = false;  // +inf takes all of the weight: the row is then read as 0 and -inf
-  auto load = [&](int i, float (&v)[kVec]) {
-    if (a.vectors && i + kVec <= seg1) {
-      const uint4 r = *reinterpret_cast<const uint4*>(x + static_cast<long long>(i) * (kBF16 ? 2 : 4));
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  // kVec elements of a 16-byte load
+  auto spread = [&](const uint4& r, float (&v)[kVec]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        if constexpr (kBF16)
-          v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-        else
-          v[e] = __uint_as_float(w[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        v[e] = __uint_as_float(0x7fffffffu);
-        if (i + e < seg1) {
-          if constexpr (kBF16)
-            v[e] = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(x)[i + e]);
-          else
-            v[e] = reinterpret_cast<const float*>(x)[i + e];
-        }
-      }
+    for (int e = 0; e < kVec; ++e) {
+      if constexpr (kBF16)
+        v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+      else
+        v[e] = __uint_as_float(w[e]);
     }
     if (inf_top) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
     }
   };
+  auto vec_at = [&](int i) {
+    return __ldg(reinterpret_cast<const uint4*>(x + static_cast<long long>(i) * (kBF16 ? 2 : 4)));
+  };
+  // the kVec elements from index i on; NaN at and past `end`: like every NaN they are below
+  // all, equal to none and of weight 0
+  auto load = [&](int i, int end, float (&v)[kVec]) {
+    if (a.vectors && i + kVec <= end) {
+      spread(vec_at(i), v);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      v[e] = __uint_as_float(0x7fffffffu);
+      if (i + e < end) {
+        if constexpr (kBF16)
+          v[e] = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(x)[i + e]);
+        else
+          v[e] = reinterpret_cast<const float*>(x)[i + e];
+        if (inf_top) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
+      }
+    }
+  };
+  // f(first index, kVec values) over [begin, end) of this warp: kBatch loads are in flight
+  // before the first is used
+  auto vectors = [&](int begin, int end, auto f) {
+    int i = begin + lane * kVec;
+    if (a.vectors)
+      for (; i - lane * kVec + kBatch * kStep <= end; i += kBatch * kStep) {
+        uint4 r[kBatch];
+#pragma unroll
+        for (int h = 0; h < kBatch; ++h) r[h] = vec_at(i + h * kStep);
+#pragma unroll
+        for (int h = 0; h < kBatch; ++h) {
+          float v[kVec];
+          spread(r[h], v);
+          f(i + h * kStep, v);
+        }
+      }
+    for (; i < end; i += kStep) {
+      float v[kVec];
+      load(i, end, v);
+      f(i, v);
+    }
+  };
   // f(index, value) over this warp's range
   auto each = [&](auto f) {
-#pragma unroll 2
-    for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
-      float v[kVec];
-      load(i, v);
+    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(i + e, v[e]);
-    }
+    });
   };
 
   // ---- 1. maximum and minimum ------------------------------------------------------------
   float mx = -INFINITY, mn = INFINITY;
-#pragma unroll 4
-  for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
-    float v[kVec];
-    load(i, v);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      mx = fmaxf(mx, v[e]);
-      mn = fminf(mn, v[e]);
-    }
-  }
+  each([&](int, float v) {
+    mx = fmaxf(mx, v);
+    mn = fminf(mn, v);
+  });
   uint32_t top_key = __reduce_max_sync(DDT_FULL_MASK, f32_key(mx));
   uint32_t low_key = __reduce_min_sync(DDT_FULL_MASK, f32_key(mn));
   if (tid == 0) {
@@ -256,7 +278,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   // ---- 2. what top-k and top-p keep -----------------------------------------------------------
   float edge = -INFINITY;
   int last = V;
-  auto kept = [&](int i, float v) { return v > edge || (v == edge && i <= last); };
+  bool all_kept = true;  // of the tokens that have weight
+  auto kept = [&](int i, float v) { return all_kept || v > edge || (v == edge && i <= last); };
   // interval of a logit: equal intervals from the maximum down to the minimum, or to where
   // weights end (the last interval takes the rest)
   const float span = fminf(top - key_f32(low_key), 28.f * temp);
@@ -274,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
     __syncthreads();
     each([&](int i, float v) {
-      const int b = kept(i, v) ? bin(v) : -1;
+      const int b = v == v && kept(i, v) ? bin(v) : -1;
       if (b >= 0) {
         if (by_weight) {
           const unsigned long long w = weight(v);
@@ -346,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     const unsigned long long above_c = s.before_c, above_w = s.before_w;
     each([&](int i, float v) {
-      if (kept(i, v) && bin_of(v) == bin) {
+      if (v == v && kept(i, v) && bin_of(v) == bin) {
         const int at = atomicAdd(&s.n_list, 1);
         if (at < kList) {
           s.list_x[at] = v;
@@ -407,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       cluster.sync();  // the lists are read; (edge, last) is there
       edge = s.edge;
       last = s.last;
+      all_kept = false;
       return;
     }
     // a long list: three steps over the bits of the key, from the top
@@ -462,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       for (int i0 = seg0; i0 < seg1; i0 += kStep) {
         const int i = i0 + lane * kVec;
         float v[kVec];
-        load(i, v);
+        load(i, seg1, v);
         int m = 0;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) m += v[e] == value && kept(i + e, v[e]);
@@ -486,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     cluster.sync();
     last = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
     edge = value;
+    all_kept = false;
     cluster.sync();  // before the next search writes again
   };
   if (k == 1) {
@@ -496,6 +521,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     if (lane == 0) atomicMin(&s.tie_index, first);
     cluster.sync();
     edge = top;
+    all_kept = false;
     last = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
   } else {
     if (k < V) cut(false, k);
@@ -504,37 +530,54 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
 
   // ---- 3. kept weight, target, token ---------------------------------------------------------
   auto kept_limbs = [&](int i, float v, uint32_t& hi, uint32_t& lo) {
-    hi = lo = 0;
-    if (kept(i, v)) {
-      const float e = expf(scaled(v));
-      if (e >= min_p) limbs(e, hi, lo);
-    }
+    const float e = expf(scaled(v));
+    const bool in = e >= min_p && kept(i, v);
+    limbs(e, hi, lo);
+    hi = in ? hi : 0;
+    lo = in ? lo : 0;
   };
-  unsigned long long mine = 0;
-#pragma unroll 2
-  for (int i = seg0 + lane * kVec; i < seg1; i += kStep) {
-    float v[kVec];
-    load(i, v);
-    uint32_t hi = 0, lo = 0;
+  // kept weight of the warp's [begin, end)
+  auto weigh = [&](int begin, int end) {
+    unsigned long long sum = 0;
+    vectors(begin, end, [&](int i, float (&v)[kVec]) {
+      uint32_t hi = 0, lo = 0;
+      bool any = all_kept;
+      if (!any) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      uint32_t h, l;
-      kept_limbs(i + e, v[e], h, l);
-      hi += h;
-      lo += l;
+        for (int e = 0; e < kVec; ++e) any |= v[e] >= edge;
+      }
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          uint32_t h, l;
+          kept_limbs(i + e, v[e], h, l);
+          hi += h;
+          lo += l;
+        }
+      }
+      sum += (static_cast<unsigned long long>(hi) << 20) + lo;
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(DDT_FULL_MASK, sum, o);
+    return sum;
+  };
+  // weight before this warp's part, of the parts of the CTA's warps in order
+  auto before_warp = [&](unsigned long long part, unsigned long long& all) {
+    __syncthreads();
+    if (lane == 0) s.warp_sum[0][warp] = part;
+    __syncthreads();
+    unsigned long long before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const unsigned long long o = s.warp_sum[0][w];
+      if (w < warp) before += o;
+      all += o;
     }
-    mine += (static_cast<unsigned long long>(hi) << 20) + lo;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(DDT_FULL_MASK, mine, o);
-  __syncthreads();
-  if (lane == 0) s.warp_sum[0][warp] = mine;
-  __syncthreads();
-  unsigned long long before = 0, all = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s.warp_sum[0][w];
-    all += s.warp_sum[0][w];
-  }
+    return before;
+  };
+  unsigned long long mine = weigh(seg0, seg1), all;
+  unsigned long long before = before_warp(mine, all);
   if (tid == 0) s.sum = all;
   cluster.sync();
   unsigned long long total = lane < ranks ? peer(lane)->sum : 0ull;
@@ -545,16 +588,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     earlier += __shfl_xor_sync(DDT_FULL_MASK, earlier, o);
   }
   total = __shfl_sync(DDT_FULL_MASK, total, 0);
-  before += __shfl_sync(DDT_FULL_MASK, earlier, 0);
+  earlier = __shfl_sync(DDT_FULL_MASK, earlier, 0);
   long long t = static_cast<long long>(floor(static_cast<double>(a.u[row]) * static_cast<double>(total)));
   t = max(min(t, static_cast<long long>(total) - 1), 0ll);
   unsigned long long target = static_cast<unsigned long long>(t);
-  if (before <= target && target < before + mine) {
-    target -= before;
-    for (int i0 = seg0; i0 < seg1; i0 += kStep) {
-      const int i = i0 + lane * kVec;
+  if (earlier <= target && target < earlier + all) {  // this CTA holds the token
+    // its warps share the range of the warp that holds it, until a warp's part is one step
+    target -= earlier;
+    int begin = seg0, end = seg1;
+    while (true) {
+      if (before <= target && target < before + mine && lane == 0) {
+        s.range0 = begin;
+        s.range1 = end;
+        s.before_w = before;
+      }
+      __syncthreads();
+      target -= s.before_w;
+      const int r0 = s.range0, r1 = s.range1;
+      if (r1 - r0 <= kStep) break;
+      const int part = ((r1 - r0 + kWarps - 1) / kWarps + kStep - 1) / kStep * kStep;
+      begin = min(r0 + warp * part, r1);
+      end = min(begin + part, r1);
+      mine = weigh(begin, end);
+      before = before_warp(mine, all);
+    }
+    if (warp == 0) {
+      const int i = s.range0 + lane * kVec;
       float v[kVec];
-      load(i, v);
+      load(i, s.range1, v);
       unsigned long long w[kVec], n = 0;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
@@ -562,34 +623,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         kept_limbs(i + e, v[e], h, l);
         n += w[e] = (static_cast<unsigned long long>(h) << 20) + l;
       }
-      unsigned long long incl = n;
+      unsigned long long at = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(DDT_FULL_MASK, incl, o);
-        if (lane >= o) incl += y;
+        const unsigned long long y = __shfl_up_sync(DDT_FULL_MASK, at, o);
+        if (lane >= o) at += y;
       }
-      const unsigned long long step = __shfl_sync(DDT_FULL_MASK, incl, 31);
-      if (target < step) {
-        unsigned long long at = incl - n;
-        if (at <= target && target < incl) {
-          int pick = 0;
-          float value = 0.f;
+      at -= n;
+      if (at <= target && target < at + n) {
+        int pick = 0;
+        float value = 0.f;
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            if (at <= target && target < at + w[e]) {
-              pick = i + e;
-              value = v[e];
-            }
-            at += w[e];
+        for (int e = 0; e < kVec; ++e) {
+          if (at <= target && target < at + w[e]) {
+            pick = i + e;
+            value = v[e];
           }
-          a.tokens[row] = pick;
-          if (a.logprobs)
-            a.logprobs[row] = static_cast<float>(static_cast<double>(scaled(value)) -
-                                                 (log(static_cast<double>(total)) - kLogUnit));
+          at += w[e];
         }
-        break;
+        a.tokens[row] = pick;
+        if (a.logprobs)
+          a.logprobs[row] = static_cast<float>(static_cast<double>(scaled(value)) -
+                                               (log(static_cast<double>(total)) - kLogUnit));
       }
-      target -= step;
     }
   }
   cluster.sync();  // no CTA leaves while another may read its shared memory
@@ -622,11 +678,11 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   if (!aligned(logits, size)) return DDT_ERR_ALIGN;
   sample::Args a{logits, static_cast<int>(vocab), row_stride, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs, aligned(logits, 16) && (row_stride * size) % 16 == 0};
-  // as many CTAs per row as keep the rows in one wave (two CTAs per SM), and no more than
-  // leave each warp one load
+  // as many CTAs per row as keep the rows in one wave (two CTAs per SM), or the rows in flight
+  // in half of L2 (they are read again), and no more than leave each thread one load
   int ranks = 1;
-  while (ranks < sample::kMaxCluster && rows * ranks * 2 <= 2 * 148 &&
-         vocab > ranks * sample::kThreads * (16 / size))
+  while (ranks < sample::kMaxCluster && vocab > ranks * sample::kThreads * (16 / size) &&
+         (rows * ranks * 2 <= 2 * 148 || 2 * 148 / ranks * vocab * size > (int64_t(64) << 20)))
     ranks *= 2;
   auto kernel = dtype == DDT_BF16 ? sample::sample_kernel<true> : sample::sample_kernel<false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
