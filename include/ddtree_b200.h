@@ -535,12 +535,10 @@ int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
  * 1e-5 keeps the first token alone.  NaN logits count as -inf; -inf tokens are never drawn; a row
  * with no other gives token -1 and logprob -inf.  vocab < 2^22.
  * Replaces sample() at temperature > 0 (model/utils.py:28-35: softmax and torch.multinomial).
- * The workspace (ddt_sample_workspace_bytes; may be 0) needs no initialisation. */
-size_t ddt_sample_workspace_bytes(int64_t rows, int64_t vocab);
+ * No workspace. */
 int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
-               const float* min_p, int64_t* tokens, float* logprobs, void* workspace,
-               size_t workspace_bytes, void* stream);
+               const float* min_p, int64_t* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -99,8 +99,7 @@ SIGNATURES = {
     "ddt_paged_attn_workspace_bytes": (_S, [_I, _I, _I, _I]),
     "ddt_paged_attn": (_i, [_P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I,
                             _I, _I, _I, _F, _P, _I, _I, _P, _S, _P, _P]),
-    "ddt_sample_workspace_bytes": (_S, [_I, _I]),
-    "ddt_sample": (_i, [_P, _i, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "ddt_sample": (_i, [_P, _i, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 

@@ -656,19 +656,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
 
 using namespace ddt;
 
-extern "C" size_t ddt_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-  (void)rows;
-  (void)vocab;
-  return 0;
-}
-
 extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t vocab,
                           int64_t row_stride, const float* u, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p,
-                          int64_t* tokens, float* logprobs, void* workspace,
-                          size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
+                          int64_t* tokens, float* logprobs, void* stream) {
   if (dtype != DDT_F32 && dtype != DDT_BF16) return DDT_ERR_DTYPE;
   if (rows < 0 || vocab <= 0 || row_stride < vocab) return DDT_ERR_INVALID;
   if (vocab >= (int64_t(1) << 22) || rows > 0x7fffffff / sample::kMaxCluster) return DDT_ERR_CAPACITY;

@@ -101,13 +101,19 @@ class _Workspaces:
 
 
 WORKSPACES = _Workspaces()
+_STATUS_WORDS: dict[int, torch.Tensor] = {}
 
 
 def attention_status(device: torch.device) -> torch.Tensor:
     """The device's default status word (i32 [1]) of tree-attention launches that are given
     none: a bounded wait of the kernel that ran out sets it non-zero."""
-    with WORKSPACES.lane(0):  # one status word per device, whatever lane a launch runs in
-        return WORKSPACES.get(device, "attn_status", 256)[:4].view(torch.int32)
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    word = _STATUS_WORDS.get(idx)
+    if word is None:
+        with WORKSPACES.lane(0):  # one status word per device, whatever lane a launch runs in
+            word = WORKSPACES.get(device, "attn_status", 256)[:4].view(torch.int32)
+        _STATUS_WORDS[idx] = word
+    return word
 
 
 STATUS_TIMEOUT = 1      # a bounded wait of a kernel ran out
@@ -876,9 +882,32 @@ class PageStep:
                         torch.empty(1, **i32))
 
 
+# These launches are short next to their host side, so its checks are kept to one call per
+# tensor and property (stride() and shape whole, get_device(), the raw stream).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
+def _device_of(*ts: torch.Tensor) -> int:
+    idx = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != idx or idx < 0:
+            _require_cuda(*ts)
+    return idx
+
+
 def _need(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
+
+
+def _table_view(block_table: torch.Tensor, requests: int) -> tuple[int, int]:
+    """(row stride, columns) of a block table i32 [requests, max_pages]."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+            block_table.shape[0] != requests or block_table.stride(1) != 1:
+        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
+    cols = block_table.shape[1]
+    return (block_table.stride(0) if requests > 1 else cols), cols
 
 
 def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -892,53 +921,48 @@ def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     out.free_count (which may be free_count; out.kv_lens may be old_lens or new_lens).
     max_tokens bounds the step's new tokens.  A step that does not fit changes nothing and
     reports itself in the status word (check_status)."""
-    dev = _require_cuda(old_lens, new_lens, block_table, free_pages, free_count)
+    idx = _device_of(old_lens, new_lens, block_table, free_pages, free_count)
     R = old_lens.numel()
     _need(old_lens, torch.int32, (R,), "old_lens")
     _need(new_lens, torch.int32, (R,), "new_lens")
     _need(free_count, torch.int32, (1,), "free_count")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R or \
-            block_table.stride(1) != 1:
-        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
+    t_stride, cols = _table_view(block_table, R)
     if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
         raise ValueError("free_pages must be a contiguous i32 vector")
     if out is None:
-        out = PageStep.allocate(dev, R, max_tokens)
+        out = PageStep.allocate(old_lens.device, R, max_tokens)
     else:
-        _require_cuda(old_lens, out.kv_lens, out.cu_new, out.slot_map, out.positions,
-                      out.free_count)
+        _device_of(old_lens, out.kv_lens, out.cu_new, out.slot_map, out.positions, out.free_count)
         _need(out.kv_lens, torch.int32, (R,), "out.kv_lens")
         _need(out.cu_new, torch.int32, (R + 1,), "out.cu_new")
         _need(out.slot_map, torch.int64, (max_tokens,), "out.slot_map")
         _need(out.positions, torch.int64, (max_tokens,), "out.positions")
         _need(out.free_count, torch.int32, (1,), "out.free_count")
     if status is None:
-        status = attention_status(dev)
+        status = attention_status(old_lens.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(dev, "page_tables", lib.ddt_page_tables_workspace_bytes(R))
+    ws = WORKSPACES.get(old_lens.device, "page_tables", lib.ddt_page_tables_workspace_bytes(R))
     check(lib.ddt_page_tables(
-        old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
-        block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], page_size,
-        free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), out.kv_lens.data_ptr(),
-        out.cu_new.data_ptr(), out.slot_map.data_ptr(), out.positions.data_ptr(), max_tokens,
-        out.free_count.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)),
-        "ddt_page_tables")
+        old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(), t_stride, cols,
+        page_size, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
+        out.kv_lens.data_ptr(), out.cu_new.data_ptr(), out.slot_map.data_ptr(),
+        out.positions.data_ptr(), max_tokens, out.free_count.data_ptr(), ws.data_ptr(),
+        ws.numel(), status.data_ptr(), _raw_stream(idx)), "ddt_page_tables")
     STATS.launches += 1
     return out
 
 
-def _pages_view(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int]:
-    """(n_pages, kv_heads, page_size, page stride, head stride, row stride) of a page pool:
-    logical [pages, kv_heads, page_size, 128] bf16 with any strides but the last."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or \
-            k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+def _pages_view(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, ...]:
+    """(n_pages, kv_heads, page_size, head_dim, page stride, head stride, row stride) of a page
+    pool: logical [pages, kv_heads, page_size, head_dim] bf16 with any strides but the last."""
+    strides = k_pages.stride()
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or strides != v_pages.stride() or \
+            strides[3] != 1:
         raise ValueError("k_pages / v_pages must be [pages, kv_heads, page_size, head_dim] with "
                          "the same strides and contiguous rows")
     if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
         raise TypeError("paged K/V are bf16")
-    n, h, ps, _ = k_pages.shape
-    sp, sh, sr, _ = k_pages.stride()
-    return n, h, ps, sp, sh, sr
+    return *k_pages.shape, *strides[:3]
 
 
 def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
@@ -949,31 +973,30 @@ def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torc
     qkv [T, (q_heads + 2 kv_heads) * 128] (bf16), K / V rows into slot slot_map[i] (i64 [>= T];
     -1 writes none) of the page pool [pages, kv_heads, page_size, 128].  rope_table i32 [T, 64]
     (ddt_rope_table).  Returns q [T, q_heads, 128]."""
-    dev = _require_cuda(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages, v_pages)
-    n_pages, hkv, ps, sp, sh, sr = _pages_view(k_pages, v_pages)
-    d = k_pages.shape[3]
+    idx = _device_of(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages, v_pages)
+    n_pages, hkv, ps, d, sp, sh, sr = _pages_view(k_pages, v_pages)
     if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or qkv.shape[1] % d:
         raise ValueError("qkv must be bf16 [tokens, heads * head_dim] with unit stride")
-    T = qkv.shape[0]
-    hq = qkv.shape[1] // d - 2 * hkv
+    T, width = qkv.shape
+    hq = width // d - 2 * hkv
     if hq <= 0:
         raise ValueError("qkv holds no query heads beside the pool's KV heads")
     if q_norm_w.dtype != torch.bfloat16 or k_norm_w.dtype != torch.bfloat16 or \
-            q_norm_w.numel() != d or k_norm_w.numel() != d:
+            q_norm_w.shape != (d,) or k_norm_w.shape != (d,):
         raise ValueError("norm weights must be bf16 [head_dim]")
     _need(rope_table, torch.int32, (T, d // 2), "rope_table")
-    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or slot_map.numel() < T or \
+    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or slot_map.shape[0] < T or \
             not slot_map.is_contiguous():
         raise ValueError("slot_map must be contiguous i64 with a slot per token")
     if out is None:
-        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=qkv.device)
     else:
         _need(out, torch.bfloat16, (T, hq, d), "out")
-        _require_cuda(qkv, out)
+        _device_of(qkv, out)
     check(_lib.load().ddt_paged_qk_norm_rope(
-        qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), T, hq, hkv, d, q_norm_w.data_ptr(),
+        qkv.data_ptr(), max(qkv.stride(0), width), T, hq, hkv, d, q_norm_w.data_ptr(),
         k_norm_w.data_ptr(), eps, rope_table.data_ptr(), slot_map.data_ptr(), out.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, sp, sh, sr, _stream(dev)),
+        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, sp, sh, sr, _raw_stream(idx)),
         "ddt_paged_qk_norm_rope")
     STATS.launches += 1
     return out
@@ -988,33 +1011,35 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (the new rows' K / V are already in the pool); max_new is the host's bound on the new
     tokens of one request.  Returns [T, q_heads, 128]; rows that no request owns are not
     written."""
-    dev = _require_cuda(q, k_pages, v_pages, block_table, cu_new, kv_lens)
-    n_pages, hkv, ps, sp, sh, sr = _pages_view(k_pages, v_pages)
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.stride(2) != 1:
+    idx = _device_of(q, k_pages, v_pages, block_table, cu_new, kv_lens)
+    n_pages, hkv, ps, d, sp, sh, sr = _pages_view(k_pages, v_pages)
+    q_strides = q.stride()
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q_strides[2] != 1:
         raise ValueError("q must be bf16 [tokens, q_heads, head_dim] with contiguous rows")
-    T, hq, d = q.shape
-    if d != k_pages.shape[3]:
+    T, hq, qd = q.shape
+    if qd != d:
         raise ValueError("q and the pages differ in head_dim")
     R = kv_lens.numel()
     _need(kv_lens, torch.int32, (R,), "kv_lens")
     _need(cu_new, torch.int32, (R + 1,), "cu_new")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R or \
-            block_table.stride(1) != 1:
-        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
+    t_stride, cols = _table_view(block_table, R)
     if out is None:
-        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
+        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
+            out.get_device() != idx:
         raise ValueError("out must be like q")
+    o_strides = out.stride()
     if status is None:
-        status = attention_status(dev)
+        status = attention_status(q.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(dev, "paged_attn", lib.ddt_paged_attn_workspace_bytes(T, max_new, hq, hkv))
+    ws = WORKSPACES.get(q.device, "paged_attn",
+                        lib.ddt_paged_attn_workspace_bytes(T, max_new, hq, hkv))
     check(lib.ddt_paged_attn(
-        q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
-        sp, sh, sr, block_table.data_ptr(), block_table.stride(0) if R > 1 else block_table.shape[1],
-        block_table.shape[1], cu_new.data_ptr(), kv_lens.data_ptr(), R, T, max_new, hq, hkv, d,
-        d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
-        ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)), "ddt_paged_attn")
+        q.data_ptr(), q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
+        ps, sp, sh, sr, block_table.data_ptr(), t_stride, cols, cu_new.data_ptr(),
+        kv_lens.data_ptr(), R, T, max_new, hq, hkv, d, d ** -0.5 if scale is None else scale,
+        out.data_ptr(), o_strides[0], o_strides[1], ws.data_ptr(), ws.numel(), status.data_ptr(),
+        _raw_stream(idx)), "ddt_paged_attn")
     STATS.launches += 1
     return out
 
@@ -1027,32 +1052,32 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
     uniforms u f32 [rows], with per-row temperature f32, top_k i32, top_p f32 and min_p f32
     (None: off).  Returns (tokens i64 [rows], logprobs f32 [rows]); -1 and -inf for a row
     without a token to draw."""
-    dev = _require_cuda(logits, u, temperature)
+    idx = _device_of(logits, u, temperature)
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("logits must be [rows, vocab] with unit stride")
     rows, vocab = logits.shape
     _need(u, torch.float32, (rows,), "u")
     _need(temperature, torch.float32, (rows,), "temperature")
+    rules = []
     for t, dt, name in ((top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
                         (min_p, torch.float32, "min_p")):
         if t is not None:
-            _require_cuda(logits, t)
+            _device_of(logits, t)
             _need(t, dt, (rows,), name)
+        rules.append(None if t is None else t.data_ptr())
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=dev)
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     else:
+        _device_of(logits, out)
         _need(out, torch.int64, (rows,), "out")
     if logprobs is None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     else:
+        _device_of(logits, logprobs)
         _need(logprobs, torch.float32, (rows,), "logprobs")
-    lib = _lib.load()
-    ws = WORKSPACES.get(dev, "sample", lib.ddt_sample_workspace_bytes(rows, vocab))
-    check(lib.ddt_sample(
+    check(_lib.load().ddt_sample(
         logits.data_ptr(), _dtype_code(logits), rows, vocab, max(logits.stride(0), vocab),
-        u.data_ptr(), temperature.data_ptr(), top_k.data_ptr() if top_k is not None else None,
-        top_p.data_ptr() if top_p is not None else None,
-        min_p.data_ptr() if min_p is not None else None, out.data_ptr(), logprobs.data_ptr(),
-        ws.data_ptr(), ws.numel(), _stream(dev)), "ddt_sample")
+        u.data_ptr(), temperature.data_ptr(), *rules, out.data_ptr(), logprobs.data_ptr(),
+        _raw_stream(idx)), "ddt_sample")
     STATS.launches += 1
     return out, logprobs

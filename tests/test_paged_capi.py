@@ -60,9 +60,8 @@ def test_paged_attention_refusals(change, code):
     assert _call("ddt_paged_attn", ATTN, ATTN_OK, **change) == code
 
 
-SAMPLE = "x dtype rows vocab rs u temp k p mp tok logp ws wsb stream"
-SAMPLE_OK = dict(x=P, dtype=1, rows=2, vocab=100, rs=100, u=P, temp=P, k=P, p=P, mp=P, tok=P, logp=P, ws=P,
-                 wsb=1 << 40, stream=None)
+SAMPLE = "x dtype rows vocab rs u temp k p mp tok logp stream"
+SAMPLE_OK = dict(x=P, dtype=1, rows=2, vocab=100, rs=100, u=P, temp=P, k=P, p=P, mp=P, tok=P, logp=P, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
