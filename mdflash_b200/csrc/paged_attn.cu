@@ -51,7 +51,6 @@ static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch,
 constexpr int kUnitRows = 2 * kBlockM;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr uint64_t kTimeoutNs = 2000000000ull;
 constexpr uint32_t kHalfBytes = kBlockM * 64 * 2;  // one 64-dim half of a 128-row tile
 constexpr uint32_t kTileBytes = 2 * kHalfBytes;    // 32 KB
 constexpr uint32_t kSmemQ = 0;                     // Q0, Q1
@@ -65,7 +64,6 @@ static_assert(kSmemFirst + (DDT_MAX_PAGED_REQUESTS + 1) * 8 + 1024 + 1024 <= 232
               "shared memory");
 constexpr uint32_t kIdescS = tc::idesc_bf16_f32(kBlockM, kBlockN, false, false);
 constexpr uint32_t kIdescPV = tc::idesc_bf16_f32(kBlockM, kHeadDim, false, true);
-constexpr int kStatusTimeout = 1;
 // of every 16 pairs of exponentials, the ones computed by the FMA-pipe polynomial beside MUFU
 constexpr uint32_t kPolyPairs = 0x1249u;
 
@@ -83,17 +81,6 @@ struct Bars {
 __device__ __forceinline__ void raise_abort(Bars& b, int32_t* status) {
   *reinterpret_cast<volatile int*>(&b.abort) = 1;
   if (status) atomicOr(status, kStatusTimeout);
-}
-
-// 4-D tiled load into this CTA's shared memory, completion counted on `bar`.
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
-                                            int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(tc::smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
-      "r"(c3)
-      : "memory");
 }
 
 // whether the item's last tile holds rows past the request's length
@@ -140,7 +127,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc::tmem_alloc(&bars.tmem_base, kTmemCols);
     tc::tmem_relinquish();
   }
-  walk_begin<kBlockN>(p, 2 * tile_tok, s_first, s_warp, piece, places, kThreads / 32);
+  walk_begin<kBlockN>(p, 2 * tile_tok, gridDim.x, s_first, s_warp, piece, places, kThreads / 32);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -590,7 +577,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // first row, tokens, head and last CTA (at most one such unit: the CTA's last item)
   if (tid == kThreads - 1)
     p.parts[blockIdx.x] = (it.slot >= 0 && (it.slot & 1) )
-                              ? make_int4(it.tok0, it.n_tok, it.h, it.last_cta)
+                              ? make_int4(it.tok0, it.n_tok, it.h, cta_of(piece, it.x_last))
                               : make_int4(0, 0, 0, -1);
   tc::tc_fence_before();
   __syncthreads();
@@ -655,45 +642,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const Par
   }
 }
 
-// ---- host -----------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
-// bf16 tensor map of `rank` dimensions (the first contiguous; strides in elements of the
-// others), 128-byte swizzle, zero fill out of bounds.
-inline int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-                    const int64_t* strides, const cuuint32_t* box) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return DDT_ERR_CUDA;
-  cuuint64_t bytes[4];
-  for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
-  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
-  const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, bytes, box, es,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? DDT_OK : DDT_ERR_ALIGN;
-}
-
 // Workspace: partial O, partial (m, l), and the record of the unit that starts in each CTA.
-constexpr size_t kPartO = size_t(2) * kMaxCtas * kUnitRows * kHeadDim * sizeof(float);
-constexpr size_t kPartMl = size_t(2) * kMaxCtas * kUnitRows * 2 * sizeof(float);
-constexpr size_t kWorkspace = kPartO + kPartMl + kMaxCtas * sizeof(int4);
+constexpr size_t kPartO = size_t(2) * kSms * kUnitRows * kHeadDim * sizeof(float);
+constexpr size_t kPartMl = size_t(2) * kSms * kUnitRows * 2 * sizeof(float);
+constexpr size_t kWorkspace = kPartO + kPartMl + kSms * sizeof(int4);
+// The long kernel's area comes after the short one's, whose counters have to stay zero.
+inline size_t workspace_bytes() { return (short_workspace_bytes() + 255) / 256 * 256 + kWorkspace; }
 
 }  // namespace paged_attn
 }  // namespace ddt
@@ -706,7 +660,8 @@ extern "C" size_t ddt_paged_attn_workspace_bytes(int64_t n_tokens, int64_t max_n
   (void)max_new;
   (void)q_heads;
   (void)kv_heads;
-  return paged_attn::kWorkspace;
+  // how units are cut depends on device-side lengths: one size for all calls
+  return paged_attn::workspace_bytes();
 }
 
 extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -736,27 +691,9 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
       q_token_stride % 8 || q_head_stride % 8 || page_stride % 8 || head_stride % 8 ||
       row_stride % 8 || o_token_stride % 8 || o_head_stride % 8)
     return DDT_ERR_ALIGN;
-  if (!workspace || workspace_bytes < kWorkspace) return DDT_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < paged_attn::workspace_bytes()) return DDT_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return DDT_ERR_ALIGN;
   const int64_t group = q_heads / kv_heads;
-  CUtensorMap tm_q, tm_k, tm_v;
-  {
-    const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
-                                static_cast<cuuint64_t>(n_tokens)};
-    const int64_t strides[2] = {q_head_stride, q_token_stride};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group),
-                               static_cast<cuuint32_t>(kBlockM / group)};
-    int rc = make_map(&tm_q, q, 3, dims, strides, box);
-    if (rc) return rc;
-    const cuuint64_t kdims[4] = {kHeadDim, static_cast<cuuint64_t>(page_size),
-                                 static_cast<cuuint64_t>(kv_heads),
-                                 static_cast<cuuint64_t>(n_pages)};
-    const int64_t kstrides[3] = {row_stride, head_stride, page_stride};
-    const cuuint32_t kbox[4] = {64, static_cast<cuuint32_t>(page_size < kBlockN ? page_size : kBlockN),
-                                1, 1};
-    if ((rc = make_map(&tm_k, k_pages, 4, kdims, kstrides, kbox))) return rc;
-    if ((rc = make_map(&tm_v, v_pages, 4, kdims, kstrides, kbox))) return rc;
-  }
   Params p;
   p.block_table = block_table;
   p.table_stride = table_stride;
@@ -776,20 +713,38 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   p.out = static_cast<__nv_bfloat16*>(out);
   p.o_token_stride = o_token_stride;
   p.o_head_stride = o_head_stride;
-  p.o_part = static_cast<float*>(workspace);
-  p.ml_part = p.o_part + kPartO / sizeof(float);
-  p.parts = reinterpret_cast<int4*>(p.ml_part + kPartMl / sizeof(float));
   p.status = status;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool few = p.max_new * group <= kShortRows;
+  const int64_t tile = few ? 64 : kBlockN;
+  CUtensorMap tm_q, tm_k, tm_v;
+  const cuuint64_t kdims[4] = {kHeadDim, static_cast<cuuint64_t>(page_size),
+                               static_cast<cuuint64_t>(kv_heads), static_cast<cuuint64_t>(n_pages)};
+  const int64_t kstrides[3] = {row_stride, head_stride, page_stride};
+  const cuuint32_t kbox[4] = {64, static_cast<cuuint32_t>(page_size < tile ? page_size : tile), 1, 1};
+  int rc = make_map(&tm_k, k_pages, 4, kdims, kstrides, kbox);
+  if (rc || (rc = make_map(&tm_v, v_pages, 4, kdims, kstrides, kbox))) return rc;
+  if (few)
+    return launch_short(p, q, q_token_stride, q_head_stride, q_heads, tm_k, tm_v, workspace, st);
+  const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
+                              static_cast<cuuint64_t>(n_tokens)};
+  const int64_t strides[2] = {q_head_stride, q_token_stride};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group),
+                             static_cast<cuuint32_t>(kBlockM / group)};
+  if ((rc = make_map(&tm_q, q, 3, dims, strides, box))) return rc;
+  p.o_part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                      (short_workspace_bytes() + 255) / 256 * 256);
+  p.ml_part = p.o_part + kPartO / sizeof(float);
+  p.parts = reinterpret_cast<int4*>(p.ml_part + kPartMl / sizeof(float));
+  p.arrived = nullptr;
   const uint32_t smem = smem_alloc(n_requests);
   if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  paged_attn_kernel<<<kMaxCtas, kThreads, smem, st>>>(tm_q, tm_k, tm_v, p);
-  const int rc = launch_status();
-  if (rc) return rc;
-  paged_merge_kernel<<<dim3(kMaxCtas, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
+  paged_attn_kernel<<<kSms, kThreads, smem, st>>>(tm_q, tm_k, tm_v, p);
+  if ((rc = launch_status())) return rc;
+  paged_merge_kernel<<<dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
                        kMergeWarps * 32, 0, st>>>(p);
   return launch_status();
 }

@@ -12,7 +12,11 @@
 // a CTA has at most one of each kind.
 #pragma once
 
+#include <cuda.h>
+#include <cuda_bf16.h>
+
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace ddt {
 namespace paged_attn {
@@ -20,7 +24,9 @@ namespace paged_attn {
 constexpr int kHeadDim = 128;
 constexpr int kMaxGroup = 64;
 constexpr int kItem = 2;
-constexpr int kMaxCtas = 148;
+constexpr int kSms = 148;
+constexpr int kStatusTimeout = 1;
+constexpr uint64_t kTimeoutNs = 2000000000ull;
 
 struct Params {
   const int32_t* block_table;
@@ -32,9 +38,10 @@ struct Params {
   float scale_log2;
   __nv_bfloat16* out;
   long long o_token_stride, o_head_stride;
-  float* o_part;   // [2 * CTAs][dim / 4][rows per unit][4]
-  float* ml_part;  // [2 * CTAs][rows per unit][2]
+  float* o_part;   // partial O of each slot
+  float* ml_part;  // [slot][rows per unit][2]: m (log2 units) and l
   int4* parts;     // [CTAs]: a unit that starts in this CTA and is finished by others
+  unsigned int* arrived;  // [CTAs]: parts written of the unit that starts in this CTA
   int32_t* status;
   unsigned long long timeout_ns;
 };
@@ -63,7 +70,7 @@ struct Item {
   int len;          // keys of the request
   int t0, nt;       // key tiles of this piece
   int slot;         // -1: the unit's only piece
-  int last_cta;     // CTA of the unit's last part (parts only)
+  long long x_first, x_last;  // positions of the unit's first and last tile
 };
 
 // The piece of the line that this CTA runs, and a warp's place in it.  Both live in shared
@@ -86,11 +93,29 @@ __device__ __forceinline__ int tiles_of(const Request& q, int tok_end) {
   return end > 0 ? (end - 1) / kTile + 1 : 0;
 }
 
+// The CTA whose piece holds position x of an item's unit, searched for from this CTA on: piece c
+// holds it when c * total < (x + 1) * ctas <= (c + 1) * total.
+__device__ __forceinline__ int cta_of(const Piece& c, long long x) {
+  int at = blockIdx.x;
+  while (at * c.total >= (x + 1) * c.ctas) --at;
+  while ((at + 1) * c.total < (x + 1) * c.ctas) ++at;
+  return at;
+}
+
+// a * b / c for factors whose product fits 32 bits or not (a 64-bit division is a few hundred
+// cycles on the way to a CTA's first load)
+__device__ __forceinline__ long long mul_div(long long a, long long b, long long c) {
+  const long long n = a * b;
+  if ((n | c) >> 32) return n / c;
+  return static_cast<uint32_t>(n) / static_cast<uint32_t>(c);
+}
+
 // Costs of the requests for one KV head into s_first [n_requests + 1] (exclusive prefix), this
-// CTA's piece, and the place of its first unit; all threads of the block call it.
+// CTA's piece of at most `most` ones, and the place of its first unit; all threads of the block
+// call it.
 template <int kTile>
-__device__ void walk_begin(const Params& p, int tokens, long long* s_first, long long* s_warp,
-                           Piece& piece, Place* places, int n_places) {
+__device__ void walk_begin(const Params& p, int tokens, long long most, long long* s_first,
+                           long long* s_warp, Piece& piece, Place* places, int n_places) {
   const int nthr = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_requests + nthr - 1) / nthr;
   const int r0 = min(tid * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
@@ -117,7 +142,7 @@ __device__ void walk_begin(const Params& p, int tokens, long long* s_first, long
     Piece c;
     c.per_head = s_first[p.n_requests];
     c.total = c.per_head * p.kv_heads;
-    c.ctas = c.total < gridDim.x ? c.total : gridDim.x;
+    c.ctas = min(min(static_cast<long long>(gridDim.x), most), c.total);
     c.x0 = c.x1 = 0;
     Place w;
     w.h = p.kv_heads;
@@ -125,9 +150,9 @@ __device__ void walk_begin(const Params& p, int tokens, long long* s_first, long
     w.u0 = 0;
     w.it.slot = -1;
     if (blockIdx.x < c.ctas) {
-      c.x0 = blockIdx.x * c.total / c.ctas;
-      c.x1 = (blockIdx.x + 1) * c.total / c.ctas;
-      w.h = static_cast<int>(c.x0 / c.per_head);
+      c.x0 = mul_div(blockIdx.x, c.total, c.ctas);
+      c.x1 = mul_div(blockIdx.x + 1, c.total, c.ctas);
+      w.h = static_cast<int>(mul_div(c.x0, 1, c.per_head));
       const long long at = c.x0 - w.h * c.per_head;
       int lo = 0, hi = p.n_requests - 1;
       while (lo < hi) {
@@ -175,13 +200,8 @@ __device__ __forceinline__ bool walk_next(const Params& p, int tokens, const lon
         w.it.t0 = lo;
         w.it.nt = hi - lo;
         w.it.slot = hi - lo == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (lo == 0 ? 1 : 0);
-        // piece c holds position x when c * total < (x + 1) * ctas <= (c + 1) * total; the
-        // unit's last position is in the piece of its last part (a search: a 64-bit division
-        // is a call, and made the whole kernel spill around it)
-        int last = blockIdx.x;
-        if (w.it.slot >= 0)
-          while ((last + 1) * c.total < (w.u0 + kItem + tiles) * c.ctas) ++last;
-        w.it.last_cta = last;
+        w.it.x_first = w.u0 + kItem;
+        w.it.x_last = w.u0 + kItem + tiles - 1;
       }
       ++w.j;
       w.u0 += kItem + tiles;
@@ -204,6 +224,61 @@ __device__ __forceinline__ bool walk_next(const Params& p, int tokens, const lon
   __syncwarp();
   return w.more != 0;
 }
+
+// 4-D tiled load into this CTA's shared memory, completion counted on `bar`.
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(tc::smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+      "r"(c3)
+      : "memory");
+}
+
+// ---- host: tensor maps ----
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  }
+  return fn;
+}
+
+// bf16 tensor map of `rank` dimensions (the first contiguous; strides in elements of the
+// others), 128-byte swizzle, zero fill out of bounds.
+inline int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+                    const int64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return DDT_ERR_CUDA;
+  cuuint64_t bytes[4];
+  for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, bytes, box, es,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DDT_OK : DDT_ERR_ALIGN;
+}
+
+// The launch of the kernel for requests of few new tokens (paged_decode.cu): all rows of a
+// request and KV head, max_new * group <= kShortRows, in one unit.
+constexpr int kShortRows = 32;
+constexpr int kShortCtas = 2 * kSms;
+size_t short_workspace_bytes();
+int launch_short(Params& p, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                 int64_t q_heads, const CUtensorMap& tm_k, const CUtensorMap& tm_v, void* workspace,
+                 cudaStream_t st);
 
 }  // namespace paged_attn
 }  // namespace ddt
