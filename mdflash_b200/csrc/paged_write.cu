@@ -8,9 +8,10 @@
 // weight and each product, as the transformers modules do; one rounding halves the error.)
 //
 // HBM-bound (12.3 KB read and written per token at 32 + 8 heads).  A warp takes some heads of one
-// token, two at a time: 16 lanes per head, 8 elements (16 bytes) each, the rotary partner 8 lanes
-// away; the token's angles and the norm weights stay in registers, four loads are in flight.
-// (One head per warp with 8-byte loads: 8191 tokens in 70 us, 2.9 TB/s.)
+// token, two at a time: 16 lanes per head, lane c the elements [4 c, 4 c + 4) and their rotary
+// partners 64 on; the token's angles and the norm weights stay in registers, eight loads are in
+// flight.  8191 tokens take 40 us, 5.0 TB/s or 0.77 of the copy rate.  (One head per warp: 70 us;
+// 16-byte loads with the partner fetched by a shuffle: 46 us; two pairs in flight: 45 us.)
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -40,17 +41,19 @@ struct WriteArgs {
 
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void spread8(const uint4& r, float (&x)[8]) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = lo_f(w[e]);
-    x[2 * e + 1] = hi_f(w[e]);
-  }
+__device__ __forceinline__ void spread4(const uint2& r, float* x) {
+  x[0] = lo_f(r.x);
+  x[1] = hi_f(r.x);
+  x[2] = lo_f(r.y);
+  x[3] = hi_f(r.y);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 constexpr int kWriteThreads = 256;
-constexpr int kBatch = 4;  // loads in flight per lane: 8 heads
+constexpr int kBatch = 4;  // pairs of heads in flight
 
 __global__ void __launch_bounds__(kWriteThreads)
 paged_write_kernel(const WriteArgs a, const int heads_per_warp, const int chunks) {
@@ -62,32 +65,29 @@ paged_write_kernel(const WriteArgs a, const int heads_per_warp, const int chunks
   const int h0 = static_cast<int>(gw - tok * chunks) * heads_per_warp;
   const int heads = a.q_heads + 2 * a.kv_heads;
   const int h1 = min(h0 + heads_per_warp, heads);
-  const int sub = lane >> 4, c = lane & 15;  // head of the pair, elements [8 c, 8 c + 8)
-  const __nv_bfloat16* src = a.qkv + tok * a.qkv_stride + c * 8;
+  const int sub = lane >> 4, c = lane & 15;  // head of the pair, elements 4 c .. and 64 + 4 c ..
+  const __nv_bfloat16* src = a.qkv + tok * a.qkv_stride + c * 4;
   const long long slot = a.slots[tok];
   const bool writes = slot >= 0 && slot < a.n_slots;
   const long long at = (slot >> a.page_shift) * a.page_stride +
-                       (slot & ((1ll << a.page_shift) - 1)) * a.row_stride + c * 8;
-  // angles of elements 8 c .. (the second half of a head has those of the first)
-  float cs[8], sn[8];
-  {
-    const uint32_t* t = a.rope + tok * (kHeadDim / 2) + (c & 7) * 8;
-    const uint4 t0 = *reinterpret_cast<const uint4*>(t), t1 = *reinterpret_cast<const uint4*>(t + 4);
-    const uint32_t w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+                       (slot & ((1ll << a.page_shift) - 1)) * a.row_stride + c * 4;
+  const uint4 angles = *reinterpret_cast<const uint4*>(a.rope + tok * (kHeadDim / 2) + c * 4);
+  const uint32_t ang[4] = {angles.x, angles.y, angles.z, angles.w};
+  uint2 qw[2], kw[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      cs[e] = lo_f(w[e]);
-      sn[e] = c < 8 ? -hi_f(w[e]) : hi_f(w[e]);
-    }
+  for (int p = 0; p < 2; ++p) {
+    qw[p] = *reinterpret_cast<const uint2*>(a.qw + p * 64 + c * 4);
+    kw[p] = *reinterpret_cast<const uint2*>(a.kw + p * 64 + c * 4);
   }
-  const uint4 qw = *reinterpret_cast<const uint4*>(a.qw + c * 8);
-  const uint4 kw = *reinterpret_cast<const uint4*>(a.kw + c * 8);
   for (int hb = h0; hb < h1; hb += 2 * kBatch) {
-    uint4 raw[kBatch];
+    uint2 raw[kBatch][2];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int h = hb + 2 * i + sub;
-      raw[i] = h < h1 ? *reinterpret_cast<const uint4*>(src + h * kHeadDim) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        raw[i][p] = h < h1 ? *reinterpret_cast<const uint2*>(src + h * kHeadDim + p * 64)
+                           : make_uint2(0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -95,29 +95,35 @@ paged_write_kernel(const WriteArgs a, const int heads_per_warp, const int chunks
       const int h = hb + 2 * i + sub;
       const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
       float x[8], w[8], ss = 0.f;
-      spread8(raw[i], x);
-      spread8(is_q ? qw : kw, w);
+      spread4(raw[i][0], x);
+      spread4(raw[i][1], x + 4);
+      spread4(is_q ? qw[0] : kw[0], w);
+      spread4(is_q ? qw[1] : kw[1], w + 4);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(DDT_FULL_MASK, ss, o);
       const float inv = rsqrtf(ss * (1.f / kHeadDim) + a.eps);
-      uint4 out = raw[i];
-      __nv_bfloat16* oe = reinterpret_cast<__nv_bfloat16*>(&out);
+      uint2 out[2] = {raw[i][0], raw[i][1]};
+      if (!is_v) {
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= inv * w[e];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float partner = __shfl_xor_sync(DDT_FULL_MASK, x[e], 8);
-        const float y = x[e] * cs[e] + partner * sn[e];
-        if (!is_v) oe[e] = __float2bfloat16_rn(y);
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[e] * (inv * w[e]), v = x[e + 4] * (inv * w[e + 4]);
+          const float cs = lo_f(ang[e]), sn = hi_f(ang[e]);
+          y[e] = u * cs - v * sn;
+          y[e + 4] = v * cs + u * sn;
+        }
+        out[0] = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+        out[1] = make_uint2(pack2(y[4], y[5]), pack2(y[6], y[7]));
       }
-      if (h >= h1) continue;
-      if (is_q)
-        *reinterpret_cast<uint4*>(a.q_out + (tok * a.q_heads + h) * kHeadDim + c * 8) = out;
-      else if (writes)
-        *reinterpret_cast<uint4*>((is_v ? a.v_pages : a.k_pages) + at +
-                                  (h - a.q_heads - (is_v ? a.kv_heads : 0)) * a.head_stride) = out;
+      if (h >= h1 || !(is_q || writes)) continue;
+      __nv_bfloat16* dst =
+          is_q ? a.q_out + (tok * a.q_heads + h) * kHeadDim + c * 4
+               : (is_v ? a.v_pages : a.k_pages) + at +
+                     (h - a.q_heads - (is_v ? a.kv_heads : 0)) * a.head_stride;
+      *reinterpret_cast<uint2*>(dst) = out[0];
+      *reinterpret_cast<uint2*>(dst + 64) = out[1];
     }
   }
 }
@@ -167,7 +173,7 @@ extern "C" int ddt_paged_qk_norm_rope(const void* qkv, int64_t qkv_stride, int64
   a.head_stride = head_stride;
   a.row_stride = row_stride;
   // few tokens: 2 heads per warp, so that they still cover the SMs; many: 24, which read the
-  // token's angles once (64 tokens of 48 heads 2.2 us in a recorded graph with 2 heads per warp)
+  // token's angles once (64 tokens of 48 heads: 2.9 us in a recorded graph)
   const int64_t heads = q_heads + 2 * kv_heads;
   const int per_warp = n_tokens * heads <= 148 * 64 * 2 ? 2 : n_tokens * heads <= 148 * 64 * 8 ? 8 : 24;
   const int64_t chunks = (heads + per_warp - 1) / per_warp;
