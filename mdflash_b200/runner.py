@@ -18,6 +18,8 @@ its bf16 rounding points but runs each layer as
 
 followed by the final norm and lm_head.  The rotary cos / sin of the forward's positions are
 built once (ddt_rope_table) and read by every layer.  It is used by TreeVerifier(fused=True).
+forward_paged runs the same layers over a paged K/V cache (paged.py), with
+ddt_paged_qk_norm_rope and ddt_paged_attn in place of the two contiguous stages.
 """
 from __future__ import annotations
 
@@ -203,6 +205,57 @@ class Qwen3VerifyRunner:
         logits = torch.empty((T, self.lm_head.shape[0]), dtype=x.dtype, device=dev)
         gemm(h, self.lm_head, logits)
         return logits
+
+    def forward_paged(self, ids: torch.Tensor, cache, step, max_new: int,
+                      rows: torch.Tensor | None = None,
+                      status: torch.Tensor | None = None) -> torch.Tensor:
+        """The causal forward of a paged step: ids i64 [T] (device), the new tokens of every
+        request in order, over `cache` (paged.PagedKVCache), whose `step` (PagedKVCache.step)
+        gives their positions and slots; max_new bounds the new tokens of one request.  Every
+        layer writes its K/V rows into the pages and attends over them.  Returns the logits
+        [len(rows), V] of the given rows (i64, device; None: all of them).  No counterpart in
+        the reference, whose prefill and decode run on one contiguous cache per request."""
+        lib = _lib.load()
+        st = self._stream()
+        n = ids.numel()
+        H, d = self.hidden, self.head_dim
+        if n > step.slot_map.numel():
+            raise ValueError(f"the step has {step.slot_map.numel()} token places, not {n}")
+        status = cache.status if status is None else status
+        x = torch.nn.functional.embedding(ids.view(-1), self.embed)
+        h = torch.empty_like(x)
+        q = torch.empty((n, self.q_heads, d), dtype=x.dtype, device=x.device)
+        attn = torch.zeros_like(q)  # rows beyond the step's tokens stay 0
+        act = torch.empty((n, self.inter), dtype=x.dtype, device=x.device)
+        rope = torch.empty((n, d // 2), dtype=torch.int32, device=x.device)
+        check(lib.ddt_rope_table(step.positions.data_ptr(), n, self.inv_freq.data_ptr(), d,
+                                 self.rope_scale, rope.data_ptr(), st), "ddt_rope_table")
+        K.STATS.launches += 1
+        delta = None
+        for li, w in enumerate(self.layers):
+            check(lib.ddt_add_rmsnorm(x.data_ptr(), delta.data_ptr() if delta is not None else None,
+                                      w["ln1"].data_ptr(), n, H, self.eps, x.data_ptr(),
+                                      h.data_ptr(), st), "ddt_add_rmsnorm")
+            qkv = torch.matmul(h, w["w_qkv"].t())
+            K.paged_qk_norm_rope(qkv, w["qn"], w["kn"], rope, step.slot_map, cache.k_pages[li],
+                                 cache.v_pages[li], self.eps, out=q)
+            K.paged_attention(q, cache.k_pages[li], cache.v_pages[li], cache.block_table,
+                              step.cu_new, step.kv_lens, max_new, scale=self.scaling, out=attn,
+                              status=status)
+            o = torch.matmul(attn.view(n, -1), w["w_o"].t())
+            check(lib.ddt_add_rmsnorm(x.data_ptr(), o.data_ptr(), w["ln2"].data_ptr(), n, H,
+                                      self.eps, x.data_ptr(), h.data_ptr(), st), "ddt_add_rmsnorm")
+            gu = torch.matmul(h, w["w_gu"].t())
+            check(lib.ddt_silu_mul(gu.data_ptr(), n, self.inter, act.data_ptr(), st),
+                  "ddt_silu_mul")
+            delta = torch.matmul(act, w["w_down"].t())
+            K.STATS.launches += 3
+        check(lib.ddt_add_rmsnorm(x.data_ptr(), delta.data_ptr(), self.final_norm.data_ptr(), n, H,
+                                  self.eps, x.data_ptr(), h.data_ptr(), st), "ddt_add_rmsnorm")
+        K.STATS.launches += 1
+        if rows is not None:
+            h = h.index_select(0, rows)
+        return torch.matmul(h, self.lm_head.t())
 
     def _feature_slots(self, features, feature_layers, n):
         """hidden-state index (transformers' hidden_states[i], i = layer id + 1) -> the
