@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t col_o(int q) { return q ? 384u : 128u; }
 
 struct Bars {
   uint64_t q_full, q_empty, k_full[kStages], v_full[kStages], k_empty[kStages],
-      v_empty[kStages], v_clean, s_full[2], p_half[2], p_full[2], o_ready[2], mma_done[2];
+      v_empty[kStages], v_clean[kStages], s_full[2], p_half[2], p_full[2], o_ready[2], mma_done[2];
   uint32_t issued[2];
   uint32_t tmem_base;
   int abort;
@@ -82,6 +82,11 @@ __device__ __forceinline__ void raise_abort(Bars& b, int32_t* status) {
   *reinterpret_cast<volatile int*>(&b.abort) = 1;
   if (status) atomicOr(status, kStatusTimeout);
 }
+
+// A unit of at most one query tile gives both tiles the same rows: tile 0 takes the even key
+// tiles of the item and tile 1 the odd ones, so that two chains of S, softmax and P V run side by
+// side; the epilogue joins them.
+__device__ __forceinline__ bool paired(const Item& it, int tile_tok) { return it.n_tok <= tile_tok; }
 
 // whether the item's last tile holds rows past the request's length
 __device__ __forceinline__ bool ragged(const Item& it) {
@@ -96,6 +101,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   __shared__ long long s_warp[kThreads / 32];
   __shared__ Piece piece;
   __shared__ Place places[kThreads / 32];
+  __shared__ float2 s_ml[2][kBlockM];  // (m, l) of a paired unit's two halves
   const uint32_t raw = tc::smem_u32(smem_raw);
   unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -105,12 +111,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (tid == 0) {
     tc::mbar_init(&bars.q_full, 1);
     tc::mbar_init(&bars.q_empty, 2);  // one commit per MMA issuer
-    tc::mbar_init(&bars.v_clean, 1);
     for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(&bars.k_full[s], 1);
       tc::mbar_init(&bars.v_full[s], 1);
       tc::mbar_init(&bars.k_empty[s], 2);
       tc::mbar_init(&bars.v_empty[s], 3);  // and warp 2
+      tc::mbar_init(&bars.v_clean[s], 1);
     }
     for (int q = 0; q < 2; ++q) {
       tc::mbar_init(&bars.s_full[q], 1);
@@ -163,7 +169,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // a query tile past the last row reads zeros
         if (lane < 4)
           tc::tma_load_3d(sQ + (lane >> 1) * kTileBytes + half * kHalfBytes, &tm_q, &bars.q_full,
-                          half * 64, it.h * p.group, it.tok0 + (lane >> 1) * tile_tok);
+                          half * 64, it.h * p.group,
+                          it.tok0 + (paired(it, tile_tok) ? 0 : (lane >> 1) * tile_tok));
         ++q_loads;
       };
       // page of this lane's box in key tile t, or n_pages (zeros) past the request's pages
@@ -251,7 +258,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             tc::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bars.v_clean);
+            if (lane == 0) tc::mbar_arrive(&bars.v_clean[st]);
           }
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&bars.v_empty[st]);
@@ -307,55 +314,111 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       };
       bool ok = true;
       uint32_t base = 0;
-      int J = 0, n_item = 0, n_ragged = 0;
+      int J = 0, Js = 0, n_item = 0;  // Js: tiles of this query tile
+      uint32_t cleaned = 0;           // phases of v_clean, a bit per stage
+      auto wait = [&](uint64_t* bar, int phase) {
+        return tc::mbar_wait_warp(bar, phase & 1, abort_flag, p.timeout_ns);
+      };
+      auto kbar = [&](int jg) { return wait(&bars.k_full[jg % kStages], jg / kStages); };
+      // V of the tile landed and, where the tile is ragged, was cleaned.  A stage is released
+      // after this, so neither barrier can get two phases ahead of a waiter.
+      auto vbar = [&](int jg, bool dirty) {
+        const int st = jg % kStages;
+        if (!wait(&bars.v_full[st], jg / kStages)) return false;
+        if (!dirty) return true;
+        const int phase = cleaned >> st;
+        cleaned ^= 1u << st;
+        return wait(&bars.v_clean[st], phase);
+      };
       while (ok && next()) {
-        if (it.nt == 0) continue;
         const int nt = it.nt;
+        if (nt == 0) continue;
         const bool tail = ragged(it);
-        if (!(ok = tc::mbar_wait_warp(&bars.q_full, n_item & 1, abort_flag, p.timeout_ns))) break;
-        if (!(ok = tc::mbar_wait_warp(&bars.k_full[J % kStages], (J / kStages) & 1, abort_flag,
-                                      p.timeout_ns)))
-          break;
-        if (!(ok = wait_turn(q == 0 ? base : base + 1))) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) {
-          issue_s(J, base + 1);
-          tc::mma_commit(&bars.k_empty[J % kStages]);
-        }
-        __syncwarp();
-        for (int j = 0; j < nt; ++j) {
-          const int jg = J + j;
-          const int st = jg % kStages;
-          const int sn = (jg + 1) % kStages;
-          const bool more = j + 1 < nt;
-          // K / V of the tile landed long before P_q(j): waited first, while the softmax runs
-          if (!(ok = tc::mbar_wait_warp(&bars.v_full[st], (jg / kStages) & 1, abort_flag,
-                                        p.timeout_ns)))
-            break;
-          if (!more && tail &&
-              !(ok = tc::mbar_wait_warp(&bars.v_clean, n_ragged & 1, abort_flag, p.timeout_ns)))
-            break;
-          if (more && !(ok = tc::mbar_wait_warp(&bars.k_full[sn], ((jg + 1) / kStages) & 1,
-                                                abort_flag, p.timeout_ns)))
-            break;
-          if (!(ok = tc::mbar_wait_warp(&bars.p_half[q], jg & 1, abort_flag, p.timeout_ns))) break;
-          if (!(ok = wait_turn(q == 0 ? base + j + 1 : base + j + 2))) break;
-          tc::tc_fence_after();
-          if (tc::elect_one()) issue_pv(jg, j, 0);
-          __syncwarp();
-          if (!(ok = tc::mbar_wait_warp(&bars.p_full[q], jg & 1, abort_flag, p.timeout_ns))) break;
-          tc::tc_fence_after();
-          if (tc::elect_one()) {
-            issue_pv(jg, j, 1);
-            tc::mma_commit(&bars.v_empty[st]);
-            if (more) {
-              issue_s(jg + 1, base + j + 2);  // reuses S_q / P_q: runs after the P V above
-              tc::mma_commit(&bars.k_empty[sn]);
-            } else {
-              *my_turns = base + j + 2;
+        if (!(ok = wait(&bars.q_full, n_item))) break;
+        if (paired(it, tile_tok)) {
+          // the other query tile's key tiles are waited for and released too, so that this
+          // warp keeps step with the stages' phases
+          for (int j = 0; ok && j < nt; ++j) {
+            const int jg = J + j, st = jg % kStages;
+            if ((j & 1) != q) {
+              if (j > 0) continue;  // released with the tile before it
+              if (!(ok = kbar(jg) && vbar(jg, tail && nt == 1))) break;
+              if (lane == 0) {
+                tc::mbar_arrive(&bars.k_empty[st]);
+                tc::mbar_arrive(&bars.v_empty[st]);
+              }
+              __syncwarp();
+              continue;
+            }
+            if (!(ok = kbar(jg))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+              issue_s(jg, base);
+              tc::mma_commit(&bars.k_empty[st]);
+            }
+            __syncwarp();
+            const bool other = j + 1 < nt;
+            if (other) {
+              if (!(ok = kbar(jg + 1))) break;
+              if (lane == 0) tc::mbar_arrive(&bars.k_empty[(jg + 1) % kStages]);
+              __syncwarp();
+            }
+            if (!(ok = vbar(jg, tail && !other))) break;
+            if (!(ok = wait(&bars.p_half[q], Js))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) issue_pv(jg, j - q, 0);
+            __syncwarp();
+            if (!(ok = wait(&bars.p_full[q], Js))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+              issue_pv(jg, j - q, 1);
+              tc::mma_commit(&bars.v_empty[st]);
+            }
+            __syncwarp();
+            ++Js;
+            if (other) {
+              if (!(ok = vbar(jg + 1, tail && j + 2 == nt))) break;
+              if (lane == 0) tc::mbar_arrive(&bars.v_empty[(jg + 1) % kStages]);
+              __syncwarp();
             }
           }
+          if (ok && lane == 0) *my_turns = base + nt + 1;
           __syncwarp();
+        } else {
+          if (!(ok = kbar(J))) break;
+          if (!(ok = wait_turn(q == 0 ? base : base + 1))) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+            issue_s(J, base + 1);
+            tc::mma_commit(&bars.k_empty[J % kStages]);
+          }
+          __syncwarp();
+          for (int j = 0; j < nt; ++j) {
+            const int jg = J + j;
+            const bool more = j + 1 < nt;
+            // K / V of the tile landed long before P_q(j): waited first, while the softmax runs
+            if (!(ok = vbar(jg, tail && !more))) break;
+            if (more && !(ok = kbar(jg + 1))) break;
+            if (!(ok = wait(&bars.p_half[q], Js))) break;
+            if (!(ok = wait_turn(q == 0 ? base + j + 1 : base + j + 2))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) issue_pv(jg, j, 0);
+            __syncwarp();
+            if (!(ok = wait(&bars.p_full[q], Js))) break;
+            tc::tc_fence_after();
+            if (tc::elect_one()) {
+              issue_pv(jg, j, 1);
+              tc::mma_commit(&bars.v_empty[jg % kStages]);
+              if (more) {
+                issue_s(jg + 1, base + j + 2);  // reuses S_q / P_q: runs after the P V above
+                tc::mma_commit(&bars.k_empty[(jg + 1) % kStages]);
+              } else {
+                *my_turns = base + j + 2;
+              }
+            }
+            __syncwarp();
+            ++Js;
+          }
         }
         // the item's S MMAs are all issued: Q may be replaced once they are done
         if (ok && tc::elect_one()) tc::mma_commit(&bars.q_empty);
@@ -363,7 +426,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         base += nt + 1;
         J += nt;
         ++n_item;
-        n_ragged += tail;
       }
       if (!ok && lane == 0) raise_abort(bars, p.status);
       // every MMA and commit of this warp is done before the CTA's barriers and TMEM go
@@ -388,13 +450,17 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int row_head = r - row_tok * p.group;
     const bool row_used = row_tok < tile_tok;
     bool ok = true;
-    int J = 0;
+    int J = 0;  // S tiles of this query tile so far
+    // (after a failed wait the walk goes on without work, so that both warpgroups meet at every
+    // barrier of the paired units)
     while (next()) {
-      const int tok = q * tile_tok + row_tok;  // token of this row within the unit
+      const bool pair = paired(it, tile_tok);
+      const int tok = (pair ? 0 : q * tile_tok) + row_tok;  // token of this row within the unit
       const bool valid = row_used && tok < it.n_tok;
       // keys this row sees: [0, lim); rows that are not stored see them all
       const int lim = valid ? it.past + tok + 1 : 0x7fffffff;
-      const int t0 = it.t0, nt = it.nt;
+      const int t0 = it.t0 + (pair ? q : 0), step = pair ? 2 : 1;
+      const int nt = pair ? (it.nt + 1 - q) >> 1 : it.nt;  // this query tile's key tiles
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; ok && j < nt; ++j) {
         const int jg = J + j;
@@ -403,7 +469,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           break;
         }
         tc::tc_fence_after();
-        const int left = lim - (t0 + j) * kBlockN;  // columns [0, left) are visible
+        const int left = lim - (t0 + j * step) * kBlockN;  // columns [0, left) are visible
         const bool masked = __any_sync(DDT_FULL_MASK, left < kBlockN);
         // the whole S row (128 fp32) comes out of TMEM in one round trip
         uint32_t sv[4][32];
@@ -510,68 +576,87 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (ok && nt > 0 &&
           !tc::mbar_wait_warp(&bars.o_ready[q], (J + nt - 1) & 1, abort_flag, p.timeout_ns))
         ok = false;
-      // warp-uniform: O holds this item's sums
-      const bool have = ok && nt > 0;
+      if (!ok && lane == 0) raise_abort(bars, p.status);
+      // warp-uniform: O holds this query tile's sums of the item
+      bool have = ok && nt > 0;
       if (have) tc::tc_fence_after();
-      const bool seen = have && m_used > -INFINITY;  // per row: some key was visible
-      if (it.slot >= 0) {
-        // a part: unnormalised O in fp32, [dim / 4][row][4] so that a warp's rows (consecutive)
-        // store 512 contiguous bytes at a time
-        const int ur = q * kBlockM + r;
-        float* op = p.o_part + static_cast<long long>(it.slot) * kUnitRows * kHeadDim + ur * 4;
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          if (have) {
-            tc::tmem_ld32(tO + c * 32, o);
-            tc::tmem_wait_ld();
-          } else {
+      float m2 = -INFINITY, l2 = 0.f;  // of the other half of a paired unit
+      if (pair) {
+        const bool seen = have && m_used > -INFINITY;
+        s_ml[q][r] = make_float2(seen ? m_used : -INFINITY, seen ? l : 0.f);
+        tc::tc_fence_before();
+        ok = tc::named_sync_and(1, 2 * kBlockM, ok);
+        tc::tc_fence_after();
+        const float2 o = s_ml[q ^ 1][r];
+        m2 = o.x;
+        l2 = o.y;
+        have = ok && it.nt > 0;
+      }
+      if (!(m_used > -INFINITY) || !ok) l = 0.f;
+      // O = w O_q + w2 O_(q ^ 1), l alike; weights of 0 where a half saw no key
+      const float M = fmaxf(m_used, m2);
+      const float w = pair ? (m_used == -INFINITY ? 0.f : tc::ex2_approx(m_used - M)) : 1.f;
+      const float w2 = m2 == -INFINITY ? 0.f : tc::ex2_approx(m2 - M);
+      l = l * w + l2 * w2;
+      const bool seen = have && M > -INFINITY;  // per row: some key was visible
+      // columns of O that this thread stores: all 128, or its warpgroup's half of a paired unit
+      const int c0 = pair ? q * 2 : 0, c1 = pair ? q * 2 + 2 : 4;
+      const int ur = (pair ? 0 : q * kBlockM) + r;
+      float* op = p.o_part + (it.slot >= 0 ? static_cast<long long>(it.slot) * kUnitRows * kHeadDim : 0ll) +
+                  ur * 4;
+      __nv_bfloat16* orow = p.out + (it.tok0 + tok) * p.o_token_stride +
+                            (it.h * p.group + row_head) * p.o_head_stride;
+      const float inv = seen && l > 0.f ? 1.f / l : 0.f;
+      for (int c = c0; c < c1; ++c) {
+        uint32_t o[32];
+        if (have) {
+          tc::tmem_ld32(tO + c * 32, o);
+          tc::tmem_wait_ld();
+        } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
-          }
-          if (valid) {
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (pair && have) {  // a half without key tiles has nothing in TMEM: select, not multiply
+          uint32_t o2[32];
+          tc::tmem_ld32(tl + col_o(q ^ 1) + c * 32, o2);
+          tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(op + ((c * 32 + e) / 4) * kUnitRows * 4) =
-                  make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 32; ++e) {
+            const float x = w > 0.f ? __uint_as_float(o[e]) * w : 0.f;
+            const float y = w2 > 0.f ? __uint_as_float(o2[e]) * w2 : 0.f;
+            o[e] = __float_as_uint(x + y);
           }
         }
-        if (valid)
-          *reinterpret_cast<float2*>(
-              p.ml_part + (static_cast<long long>(it.slot) * kUnitRows + ur) * 2) =
-              make_float2(seen ? m_used : -INFINITY, seen ? l : 0.f);
-      } else {
-        const float inv = seen && l > 0.f ? 1.f / l : 0.f;
-        __nv_bfloat16* orow = p.out + (it.tok0 + tok) * p.o_token_stride +
-                              (it.h * p.group + row_head) * p.o_head_stride;
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          if (have) {
-            tc::tmem_ld32(tO + c * 32, o);
-            tc::tmem_wait_ld();
-          } else {
+        if (!valid) continue;
+        if (it.slot >= 0) {
+          // a part: unnormalised O in fp32, [dim / 4][row][4] so that a warp's rows
+          // (consecutive) store 512 contiguous bytes at a time
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
-          }
-          if (valid) {
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(op + ((c * 32 + e) / 4) * kUnitRows * 4) =
+                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 v;
-              v.x = tc::pack_bf16x2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              v.y = tc::pack_bf16x2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              v.z = tc::pack_bf16x2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              v.w = tc::pack_bf16x2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(orow + c * 32 + e) = v;
-            }
+          for (int e = 0; e < 32; e += 8) {
+            uint4 v;
+            v.x = tc::pack_bf16x2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            v.y = tc::pack_bf16x2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            v.z = tc::pack_bf16x2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            v.w = tc::pack_bf16x2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(orow + c * 32 + e) = v;
           }
         }
       }
+      if (it.slot >= 0 && valid && (!pair || q == 0))
+        *reinterpret_cast<float2*>(p.ml_part +
+                                   (static_cast<long long>(it.slot) * kUnitRows + ur) * 2) =
+            make_float2(seen ? M : -INFINITY, seen ? l : 0.f);
       // the O columns are read: the next item's first P V MMA may overwrite them (it waits
-      // for this warpgroup's p_half of that item, which comes after this point)
+      // for p_half of that item, which comes after this point, from either warpgroup)
       tc::tc_fence_before();
+      if (pair) tc::named_sync(1, 2 * kBlockM);
       J += nt;
-      if (!ok) break;
     }
-    if (!ok && lane == 0) raise_abort(bars, p.status);
   }
   // what the merge kernel needs of a unit that starts in this CTA and ends in another: its
   // first row, tokens, head and last CTA (at most one such unit: the CTA's last item)
