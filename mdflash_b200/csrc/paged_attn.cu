@@ -138,6 +138,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
+  // the merge kernel may be scheduled from here on (it waits for this grid's end)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   volatile int* abort_flag = &bars.abort;
   const Item& it = places[warp].it;  // the warp's current item
   auto next = [&] { return walk_next<kBlockN>(p, 2 * tile_tok, s_first, piece, places[warp]); };
@@ -670,6 +672,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, kTmemCols);
   }
+  // a short kernel launched before this one is over before this one is: what follows in the
+  // stream waits for this one only
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- merge of the parts ----------------------------------------------------------------
@@ -681,6 +686,8 @@ constexpr int kMergeWarps = 8;
 
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const Params p) {
   const int c0 = blockIdx.x;
+  // launched while the attention kernel still runs: its writes are there after this wait
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 part = p.parts[c0];
   if (part.w < 0) return;
   const int w = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -801,17 +808,35 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   p.status = status;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Which kernel takes which request: few rows go to the short one, the rest to this one, and
+  // a batch of long chunks with single tokens between them to both.  The host knows only the
+  // longest request, so the others are judged by their mean: where they are not 16 rows or
+  // fewer, or too few to fill the SMs, this kernel takes all.  LATER
   const bool few = p.max_new * group <= kShortRows;
-  const int64_t tile = few ? 64 : kBlockN;
+  const int64_t others = n_requests - 1, one_tile = 16 / group;
+  const bool both = !few && others * kv_heads >= kSms && n_tokens - p.max_new <= one_tile * others;
   CUtensorMap tm_q, tm_k, tm_v;
   const cuuint64_t kdims[4] = {kHeadDim, static_cast<cuuint64_t>(page_size),
                                static_cast<cuuint64_t>(kv_heads), static_cast<cuuint64_t>(n_pages)};
   const int64_t kstrides[3] = {row_stride, head_stride, page_stride};
-  const cuuint32_t kbox[4] = {64, static_cast<cuuint32_t>(page_size < tile ? page_size : tile), 1, 1};
-  int rc = make_map(&tm_k, k_pages, 4, kdims, kstrides, kbox);
-  if (rc || (rc = make_map(&tm_v, v_pages, 4, kdims, kstrides, kbox))) return rc;
-  if (few)
-    return launch_short(p, q, q_token_stride, q_head_stride, q_heads, tm_k, tm_v, workspace, st);
+  auto kv_maps = [&](int64_t tile) {
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page_size < tile ? page_size : tile), 1, 1};
+    const int e = make_map(&tm_k, k_pages, 4, kdims, kstrides, box);
+    return e ? e : make_map(&tm_v, v_pages, 4, kdims, kstrides, box);
+  };
+  int rc;
+  p.from_new = 1;
+  p.to_new = p.max_new;
+  if (few || both) {
+    if (both) p.to_new = static_cast<int>(one_tile);
+    if ((rc = kv_maps(64)) ||
+        (rc = launch_short(p, q, q_token_stride, q_head_stride, q_heads, tm_k, tm_v, workspace, st)) ||
+        few)
+      return rc;
+    p.from_new = p.to_new + 1;
+    p.to_new = p.max_new;
+  }
+  if ((rc = kv_maps(kBlockN))) return rc;
   const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
                               static_cast<cuuint64_t>(n_tokens)};
   const int64_t strides[2] = {q_head_stride, q_token_stride};
@@ -827,9 +852,30 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  paged_attn_kernel<<<kSms, kThreads, smem, st>>>(tm_q, tm_k, tm_v, p);
-  if ((rc = launch_status())) return rc;
-  paged_merge_kernel<<<dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
-                       kMergeWarps * 32, 0, st>>>(p);
-  return launch_status();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  // beside the short kernel's last CTAs: the two share no output
+  cfg.numAttrs = both ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, paged_attn_kernel, tm_q, tm_k, tm_v, p) != cudaSuccess) {
+    cudaGetLastError();
+    return DDT_ERR_CUDA;
+  }
+  // programmatic launch: the merge's CTAs take the SMs as the attention's leave them and wait
+  // there for its end, instead of being launched after it
+  cfg.gridDim = dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps);
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged_merge_kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return DDT_ERR_CUDA;
+  }
+  return DDT_OK;
 }

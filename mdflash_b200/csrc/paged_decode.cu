@@ -189,6 +189,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   walk_begin<kKeys>(p, unit_tok, static_cast<long long>(kMaxParts / kM) * p.kv_heads * p.n_requests,
                     s_first, s_warp, piece, places, kConsumers + 1);
   __syncthreads();
+  // the other kernel of a mixed batch may take the SMs that this one leaves
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   volatile int* abort_flag = &bars.abort;
   const Item& it = places[warp].it;
   auto next = [&] { return walk_next<kKeys>(p, unit_tok, s_first, piece, places[warp]); };
@@ -516,8 +518,7 @@ int launch_short(Params& p, const void* q, int64_t q_token_stride, int64_t q_hea
   p.ml_part = p.o_part + kShortPartO / sizeof(float);
   p.arrived = reinterpret_cast<unsigned int*>(p.ml_part + kShortPartMl / sizeof(float));
   p.parts = nullptr;
-  const int rows = p.max_new * p.group;
-  const int m = rows <= 16 ? 1 : 2;
+  const int m = p.to_new * p.group <= 16 ? 1 : 2;
   CUtensorMap tm_q;
   const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
                               static_cast<cuuint64_t>(p.n_tokens)};

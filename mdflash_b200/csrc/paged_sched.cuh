@@ -35,6 +35,7 @@ struct Params {
   const int32_t* cu_new;
   const int32_t* kv_lens;
   int n_requests, n_tokens, max_new, group, kv_heads;
+  int from_new, to_new;  // the launch takes the requests with so many new tokens
   float scale_log2;
   __nv_bfloat16* out;
   long long o_token_stride, o_head_stride;
@@ -46,8 +47,8 @@ struct Params {
   unsigned long long timeout_ns;
 };
 
-// First query row, new tokens and key count of request r; no tokens (and the status bit, from
-// one CTA) where they are out of range.
+// First query row, new tokens and key count of request r; no tokens where another launch takes
+// the request, or (and the status bit, from one CTA) where they are out of range.
 struct Request {
   int first, n, len;
 };
@@ -58,7 +59,8 @@ __device__ __forceinline__ Request request(const Params& p, int r) {
   q.len = p.kv_lens[r];
   const bool fine = q.first >= 0 && end >= q.first && end <= p.n_tokens &&
                     end - q.first <= p.max_new && q.len >= 0 && q.len <= p.max_keys;
-  q.n = fine ? end - q.first : 0;
+  const int n = end - q.first;
+  q.n = fine && n >= p.from_new && n <= p.to_new ? n : 0;
   if (!fine && p.status && blockIdx.x == 0) atomicOr(p.status, DDT_STATUS_PAGED_RANGE);
   return q;
 }
