@@ -7,13 +7,16 @@
 //
 // A row is shared by a cluster of 1 to 8 CTAs; every warp owns a contiguous range of indices and
 // reads it with 16-byte loads in every pass (the first from HBM, the others from L2):
-//   1. maximum and minimum
-//   2. for top-k (by counts), then for top-p (by weights, of what top-k keeps): a histogram of
-//      the row over 2048 equal intervals of the logits, added over the cluster through
-//      distributed shared memory; the interval that holds the boundary; a pass that lists its
-//      tokens (a few hundred of 152k where the row looks like a model's); and every listed token
-//      compared with every other, which gives each its exact count and weight before it.  Lists of
-//      more than 1024 tokens (long runs of equal logits) are searched by the bits of the key.
+//   1. the maximum (and, where the row is truncated, the minimum)
+//   2. top-k and top-p: counts of the row over 2048 equal intervals of the logits, added over
+//      the cluster through distributed shared memory (for top-p alone also the row's weight)
+//      - top-k: the interval that holds token number k; all tokens down to it are listed (some
+//        tens or hundreds of 152k) and sorted, and the rest happens on the list
+//      - top-p alone: the interval where the running weight should reach top_p, judged by the
+//        intervals' counts and middles; the tokens of it and its neighbours are listed and
+//        sorted, the ones above weighed, and the boundary taken from the exact sums
+//      - where a list is too long (a large k, long runs of equal logits) or the boundary lies
+//        outside it: exact weights per interval, and a search by the bits of the key
 //   3. the weight of the kept tokens; the warps of the CTA that holds the target share the
 //      range of the warp that holds it, until that is one load per lane
 // CTAs exchange values through distributed shared memory, with one cluster barrier each time.
@@ -27,12 +30,17 @@ namespace sample {
 
 namespace cg = cooperative_groups;
 
+// (the row's passes are lambdas over its elements; out of line their captures would live in
+// local memory)
+#define DDT_INLINE __attribute__((always_inline))
+
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
 constexpr int kOwn = kBins / kThreads;  // bins per thread
-constexpr int kList = 1024;
+constexpr int kList = 2048;
+constexpr int kPer = kList / kThreads;  // listed tokens per thread
 constexpr double kLogUnit = 27.725887222397812;  // 40 ln 2
 
 struct Args {
@@ -85,21 +93,48 @@ __device__ __forceinline__ unsigned long long whole(float e) {
 // What a CTA shows to the others of its cluster, and its own scratch.
 struct Shared {
   alignas(16) uint32_t count[kBins], lo[kBins], hi[kBins];  // weight of a bin: hi * 2^32 + lo
-  float list_x[kList];                                      // this CTA's part of a list
-  int list_i[kList];
-  float all_x[kList];  // the cluster's list
-  int all_i[kList];
-  unsigned long long all_w[kList];
+  unsigned long long list[kList];  // this CTA's part of a list (ordered())
+  unsigned long long all[kList];   // the cluster's list
   unsigned long long warp_sum[2][kWarps];
-  unsigned long long sum;  // kept weight of the CTA
+  unsigned long long sum, above;  // weights of the CTA
   uint32_t top_key, low_key;
   int n_list, ties, tie_index;
   // found by one thread of the CTA for all of its threads
-  int bin;
+  int bin, window, kept, range0, range1;
   unsigned long long before_c, before_w, bin_c;
-  float edge;
-  int last, range0, range1;
 };
+
+// A token as a whole number: larger for a larger logit, then for a smaller index.
+__device__ __forceinline__ unsigned long long ordered(float v, int i) {
+  return (static_cast<unsigned long long>(f32_key(v)) << 32) | static_cast<uint32_t>(~i);
+}
+__device__ __forceinline__ float value_of(unsigned long long t) {
+  return key_f32(static_cast<uint32_t>(t >> 32));
+}
+__device__ __forceinline__ int index_of(unsigned long long t) {
+  return static_cast<int>(~static_cast<uint32_t>(t));
+}
+
+// Bitonic sort of n <= kList numbers above 0 in descending order by the whole block; places from
+// n to the next power of two become 0.
+__device__ __forceinline__ void sort_descending(unsigned long long* a, int n) {
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int j = n + threadIdx.x; j < size; j += kThreads) a[j] = 0ull;
+  __syncthreads();
+  for (int run = 2; run <= size; run <<= 1)
+    for (int d = run >> 1; d > 0; d >>= 1) {
+      for (int t = threadIdx.x; t < size >> 1; t += kThreads) {
+        const int i = 2 * t - (t & (d - 1)), j = i + d;
+        const unsigned long long x = a[i], y = a[j];
+        if ((x < y) == ((i & run) == 0)) {
+          a[i] = y;
+          a[j] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
 
 // Exclusive block scan of (c, w) in thread order; returns the totals too.
 __device__ __forceinline__ void scan2(unsigned long long c, unsigned long long w, Shared& s,
@@ -140,7 +175,6 @@ template <bool kBF16>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   constexpr int kVec = kBF16 ? 8 : 4;  // elements per 16-byte load
   constexpr int kStep = 32 * kVec;
-  constexpr int kBatch = 4;
   extern __shared__ unsigned char smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -150,16 +184,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   const char* x = static_cast<const char*>(a.logits) + row * a.row_stride * (kBF16 ? 2 : 4);
   auto peer = [&](int r) { return cluster.map_shared_rank(&s, r); };
 
+  // ---- the row's rules --------------------------------------------------------------------
+  const float temp_in = a.temperature[row];
+  const bool greedy = !(temp_in >= 1e-5f);
+  const float temp = greedy ? 1.f : temp_in;
+  const float p_in = a.top_p && !greedy ? a.top_p[row] : 1.f;
+  const int k_in = a.top_k ? a.top_k[row] : 0;
+  const int k = greedy || p_in <= 0.f ? 1 : (k_in > 0 && k_in < V ? k_in : V);
+  const double p = k > 1 ? static_cast<double>(p_in) : 1.0;
+  const float min_p = a.min_p && !greedy ? fminf(a.min_p[row], 1.f) : 0.f;
+  const Divisor by_temp(temp);
+
+  // ---- reading ------------------------------------------------------------------------------
   // this warp's range of indices
   const int per_warp =
       ((V + ranks * kWarps - 1) / (ranks * kWarps) + kStep - 1) / kStep * kStep;
   const int seg0 = min(static_cast<long long>(rank * kWarps + warp) * per_warp,
                        static_cast<long long>(V));
   const int seg1 = min(seg0 + per_warp, V);
-
   bool inf_top = false;  // +inf takes all of the weight: the row is then read as 0 and -inf
   // kVec elements of a 16-byte load
-  auto spread = [&](const uint4& r, float (&v)[kVec]) {
+  auto spread = [&](const uint4& r, float (&v)[kVec]) DDT_INLINE {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
@@ -173,12 +218,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       for (int e = 0; e < kVec; ++e) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
     }
   };
-  auto vec_at = [&](int i) {
+  auto vec_at = [&](int i) DDT_INLINE {
     return __ldg(reinterpret_cast<const uint4*>(x + static_cast<long long>(i) * (kBF16 ? 2 : 4)));
   };
   // the kVec elements from index i on; NaN at and past `end`: like every NaN they are below
   // all, equal to none and of weight 0
-  auto load = [&](int i, int end, float (&v)[kVec]) {
+  auto load = [&](int i, int end, float (&v)[kVec]) DDT_INLINE {
     if (a.vectors && i + kVec <= end) {
       spread(vec_at(i), v);
       return;
@@ -197,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   };
   // f(first index, kVec values) over [begin, end) of this warp: kBatch loads are in flight
   // before the first is used
-  auto vectors = [&](int begin, int end, auto f) {
+  auto vectors = [&](int begin, int end, auto f) DDT_INLINE {
+    constexpr int kBatch = 4;
     int i = begin + lane * kVec;
     if (a.vectors)
       for (; i - lane * kVec + kBatch * kStep <= end; i += kBatch * kStep) {
@@ -218,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
   };
   // f(index, value) over this warp's range
-  auto each = [&](auto f) {
+  auto each = [&](auto f) DDT_INLINE {
     vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(i + e, v[e]);
@@ -227,10 +273,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
 
   // ---- 1. maximum and minimum ------------------------------------------------------------
   float mx = -INFINITY, mn = INFINITY;
-  each([&](int, float v) {
-    mx = fmaxf(mx, v);
-    mn = fminf(mn, v);
-  });
+  if (k < V || p < 1.0) {
+    each([&](int, float v) {
+      mx = fmaxf(mx, v);
+      mn = fminf(mn, v);
+    });
+  } else {
+    each([&](int, float v) { mx = fmaxf(mx, v); });
+  }
   uint32_t top_key = __reduce_max_sync(DDT_FULL_MASK, f32_key(mx));
   uint32_t low_key = __reduce_min_sync(DDT_FULL_MASK, f32_key(mn));
   if (tid == 0) {
@@ -261,31 +311,89 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     low_key = f32_key(-INFINITY);
   }
 
-  const float temp_in = a.temperature[row];
-  const bool greedy = !(temp_in >= 1e-5f);
-  const float temp = greedy ? 1.f : temp_in;
-  const float p_in = a.top_p && !greedy ? a.top_p[row] : 1.f;
-  const int k_in = a.top_k ? a.top_k[row] : 0;
-  const int k = greedy || p_in <= 0.f ? 1 : (k_in > 0 && k_in < V ? k_in : V);
-  const double p = k > 1 ? static_cast<double>(p_in) : 1.0;
-  const float min_p = a.min_p && !greedy ? fminf(a.min_p[row], 1.f) : 0.f;
-  const Divisor by_temp(temp);
+  // ---- weights ------------------------------------------------------------------------------
   // exp of the scaled distance to the maximum, by CUDA's expf; -200 stands for all that is
   // far below a weight of 1 and for the NaN of -inf and NaN logits
   auto scaled = [&](float v) { return fmaxf(by_temp(v - top), -200.f); };
   auto weight = [&](float v) { return whole(expf(scaled(v))); };
-
-  // ---- 2. what top-k and top-p keep -----------------------------------------------------------
+  // what is kept: the logits above `edge`, and the equal ones up to index `last`
   float edge = -INFINITY;
   int last = V;
   bool all_kept = true;  // of the tokens that have weight
   auto kept = [&](int i, float v) { return all_kept || v > edge || (v == edge && i <= last); };
+  auto warp_total = [&](unsigned long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(DDT_FULL_MASK, v, o);
+    return v;
+  };
+  // sum of `part` over the CTA's warps before this one, and over all of them
+  auto before_warp = [&](unsigned long long part, unsigned long long& all) {
+    __syncthreads();
+    if (lane == 0) s.warp_sum[0][warp] = part;
+    __syncthreads();
+    unsigned long long before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const unsigned long long o = s.warp_sum[0][w];
+      if (w < warp) before += o;
+      all += o;
+    }
+    return before;
+  };
+  // sum over the cluster's CTAs of a value that they published, and over those before this one
+  auto cluster_total = [&](unsigned long long mine_at_lane, unsigned long long& earlier) {
+    unsigned long long total = lane < ranks ? mine_at_lane : 0ull;
+    earlier = lane < rank ? total : 0ull;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(DDT_FULL_MASK, total, o);
+      earlier += __shfl_xor_sync(DDT_FULL_MASK, earlier, o);
+    }
+    earlier = __shfl_sync(DDT_FULL_MASK, earlier, 0);
+    return __shfl_sync(DDT_FULL_MASK, total, 0);
+  };
+
+  // ---- the draw -------------------------------------------------------------------------------
+  // floor(u * total), at most total - 1
+  auto target_of = [&](unsigned long long total) {
+    const long long t =
+        static_cast<long long>(floor(static_cast<double>(a.u[row]) * static_cast<double>(total)));
+    return static_cast<unsigned long long>(max(min(t, static_cast<long long>(total) - 1), 0ll));
+  };
+  auto write = [&](float v, int i, unsigned long long total) {
+    a.tokens[row] = i;
+    if (a.logprobs)
+      a.logprobs[row] = static_cast<float>(static_cast<double>(scaled(v)) -
+                                           (log(static_cast<double>(total)) - kLogUnit));
+  };
+
+  // ---- 2. what top-k and top-p keep -----------------------------------------------------------
   // interval of a logit: equal intervals from the maximum down to the minimum, or to where
   // weights end (the last interval takes the rest)
   const float span = fminf(top - key_f32(low_key), 28.f * temp);
   const float per_unit = span > 0.f ? (kBins - 1) / span : 0.f;
+  auto place_of = [&](float v) { return __fmul_rn(__fsub_rn(top, v), per_unit); };
+  // (adding 2^23 with rounding toward zero leaves the whole part in the low bits, at four times
+  // the rate of a conversion; of NaN it makes the last interval)
   auto bin_of = [&](float v) {
-    return min(__float2int_rz(__fmul_rn(__fsub_rn(top, v), per_unit)), kBins - 1);
+    return static_cast<int>(__float_as_uint(__fadd_rz(fminf(place_of(v), kBins - 1.f), 8388608.f)) -
+                            0x4b000000u);
+  };
+  auto clear = [&] {
+    for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
+    if (tid == 0) {
+      s.bin = -1;
+      s.n_list = s.window = 0;
+    }
+    __syncthreads();
+  };
+  // counts of this thread's kOwn bins b0 .. over the cluster
+  auto bin_counts = [&](int b0, unsigned long long (&c)[kOwn]) {
+    for (int r = 0; r < ranks; ++r) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&peer(r)->count[b0]);
+      c[0] += o.x, c[1] += o.y, c[2] += o.z, c[3] += o.w;
+    }
   };
   // Histogram of the kept tokens by `bin` (those with a bin >= 0), added over the cluster; then
   // the bin that holds the boundary: by weight the last one whose weight before it is below
@@ -293,9 +401,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   double reach = 0.0;
   auto boundary = [&](bool by_weight, bool count, bool ascending, unsigned long long want,
                       unsigned long long above_c, unsigned long long above_w, bool set_reach,
-                      auto bin) {
-    for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
-    __syncthreads();
+                      auto bin) DDT_INLINE {
+    clear();
     each([&](int i, float v) {
       const int b = v == v && kept(i, v) ? bin(v) : -1;
       if (b >= 0) {
@@ -310,18 +417,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         if (count) atomicAdd(&s.count[b], 1u);
       }
     });
-    if (tid == 0) s.bin = -1;
     cluster.sync();
     // thread t owns kOwn bins, in the order of the tokens
     unsigned long long c[kOwn] = {}, w[kOwn] = {}, c_sum = 0, w_sum = 0;
     const int b0 = (ascending ? tid : kThreads - 1 - tid) * kOwn;
-    for (int r = 0; r < ranks; ++r) {
-      const Shared* o = peer(r);
-      if (count) {
-        const uint4 oc = *reinterpret_cast<const uint4*>(&o->count[b0]);
-        c[0] += oc.x, c[1] += oc.y, c[2] += oc.z, c[3] += oc.w;
-      }
-      if (by_weight) {
+    if (count) bin_counts(b0, c);
+    if (by_weight)
+      for (int r = 0; r < ranks; ++r) {
+        const Shared* o = peer(r);
         const uint4 ol = *reinterpret_cast<const uint4*>(&o->lo[b0]),
                     oh = *reinterpret_cast<const uint4*>(&o->hi[b0]);
         w[0] += (static_cast<unsigned long long>(oh.x) << 32) + ol.x;
@@ -329,7 +432,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         w[2] += (static_cast<unsigned long long>(oh.z) << 32) + ol.z;
         w[3] += (static_cast<unsigned long long>(oh.w) << 32) + ol.w;
       }
-    }
 #pragma unroll
     for (int h = 0; h < kOwn; ++h) {
       c_sum += c[h];
@@ -357,10 +459,224 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     __syncthreads();
   };
+  // this CTA's part of a list, as far as it fits
+  auto append = [&](int i, float v) {
+    const int at = atomicAdd(&s.n_list, 1);
+    if (at < kList) s.list[at] = ordered(v, i);
+  };
+  // The cluster's list into s.all, in any order; its length (nothing is copied above kList).
+  auto gather = [&] {
+    const int mine = lane < ranks ? peer(lane)->n_list : 0;
+    const int n = __reduce_add_sync(DDT_FULL_MASK, mine);
+    if (n > kList) return n;
+    for (int r = 0, at = 0; r < ranks; ++r) {
+      const unsigned long long* o = peer(r)->list;
+      const int m = __shfl_sync(DDT_FULL_MASK, mine, r);
+      for (int j = tid; j < m; j += kThreads) s.all[at + j] = o[j];
+      at += m;
+    }
+    __syncthreads();
+    return n;
+  };
+  // weights before this thread's kPer tokens of the sorted s.all, and of all n
+  auto running = [&](int n, unsigned long long (&w)[kPer], unsigned long long& all) {
+    unsigned long long sum = 0, c0, before;
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int j = tid * kPer + h;
+      w[h] = sum;
+      if (j < n) sum += weight(value_of(s.all[j]));
+    }
+    scan2(0ull, sum, s, c0, before, all);
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) w[h] += before;
+  };
+  // Moves (edge, last) to the last token of the sorted s.all that keep(number in the list, weight
+  // before it) holds for: a prefix of it, and at least the first.  Returns how many.
+  auto settle = [&](int n, const unsigned long long (&w)[kPer], auto keep) {
+    int held = 0;
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int j = tid * kPer + h;
+      held += j < n && keep(j, w[h]);
+    }
+    held = __reduce_add_sync(DDT_FULL_MASK, held);
+    if (tid == 0) s.kept = 0;
+    __syncthreads();
+    if (lane == 0) atomicAdd(&s.kept, held);
+    __syncthreads();
+    const int m = s.kept;
+    edge = value_of(s.all[m - 1]);
+    last = index_of(s.all[m - 1]);
+    all_kept = false;
+    return m;
+  };
+
+  // top-k on a list of all candidates, by the first CTA: false, and nothing done, where the
+  // list would be too long.
+  auto by_list = [&]() -> bool {
+    boundary(false, true, true, k, 0, 0, false, bin_of);
+    const int bin = s.bin;
+    // (without a bin there are fewer tokens than k, NaN being none)
+    const bool fits = bin >= 0 && s.before_c + s.bin_c <= kList;
+    if (!fits) {
+      cluster.sync();  // the histograms are read
+      return false;
+    }
+    const float past = bin + 1.f;
+    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
+      float top_of = v[0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) top_of = fmaxf(top_of, v[e]);
+      if (!(place_of(top_of) < past)) return;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (place_of(v[e]) < past) append(i + e, v[e]);
+    });
+    cluster.sync();
+    const int listed = rank == 0 ? gather() : 0;
+    cluster.sync();  // the lists are read
+    if (rank != 0) return true;
+    sort_descending(s.all, listed);
+    const int n = min(listed, k);
+    unsigned long long w[kPer], all;
+    running(n, w, all);
+    const double limit = p * static_cast<double>(all);
+    // the kept ones, as (~index | key), to be drawn from in the order of the indices
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int j = tid * kPer + h;
+      if (j >= n) continue;
+      const unsigned long long t = s.all[j];
+      const bool in = (j == 0 || !(p < 1.0) || static_cast<double>(w[h]) < limit) &&
+                      expf(scaled(value_of(t))) >= min_p;
+      s.list[j] = in ? (t << 32) | (t >> 32) : 0ull;
+    }
+    __syncthreads();
+    sort_descending(s.list, n);
+    unsigned long long own[kPer], sum = 0, c0, before, total;
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int j = tid * kPer + h;
+      const unsigned long long t = j < n ? s.list[j] : 0ull;
+      own[h] = t ? weight(key_f32(static_cast<uint32_t>(t))) : 0ull;
+      sum += own[h];
+    }
+    scan2(0ull, sum, s, c0, before, total);
+    const unsigned long long target = target_of(total);
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      if (before <= target && target < before + own[h]) {
+        const unsigned long long t = s.list[tid * kPer + h];
+        write(key_f32(static_cast<uint32_t>(t)), static_cast<int>(~static_cast<uint32_t>(t >> 32)),
+              total);
+      }
+      before += own[h];
+    }
+    return true;
+  };
+
+  // top-p alone: (edge, last), and the weight that this warp's range keeps.  False, and nothing
+  // done, where the intervals' middles mislead or a list would be too long.
+  auto nucleus = [&](unsigned long long& mine) -> bool {
+    clear();
+    unsigned long long sum = 0, all, earlier;
+    vectors(seg0, seg1, [&](int, float (&v)[kVec]) {
+      uint32_t hi = 0, lo = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (v[e] == v[e]) atomicAdd(&s.count[bin_of(v[e])], 1u);
+        uint32_t h, l;
+        limbs(expf(scaled(v[e])), h, l);
+        hi += h;
+        lo += l;
+      }
+      sum += (static_cast<unsigned long long>(hi) << 20) + lo;
+    });
+    before_warp(warp_total(sum), all);
+    if (tid == 0) s.sum = all;
+    cluster.sync();
+    const unsigned long long whole_row =
+        cluster_total(lane < ranks ? peer(lane)->sum : 0ull, earlier);
+    reach = p * static_cast<double>(whole_row);
+    unsigned long long c[kOwn] = {}, w[kOwn], c_sum = 0, w_sum = 0, c0, w0, w_all;
+    const int b0 = tid * kOwn;
+    bin_counts(b0, c);
+    const float width = per_unit > 0.f ? 1.f / per_unit : 0.f;
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      w[h] = c[h] * whole(expf(scaled(top - (b0 + h + 0.5f) * width)));
+      c_sum += c[h];
+      w_sum += w[h];
+    }
+    scan2(c_sum, w_sum, s, c0, w0, w_all);
+    // judged from the row's end: what follows the boundary is many light tokens, whose
+    // distances from their intervals' middles cancel; a heavy token's would not
+    double from = static_cast<double>(whole_row) - static_cast<double>(w_all - w0);
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      const double to = from + static_cast<double>(w[h]);
+      if (from < reach && !(to < reach)) s.bin = b0 + h;
+      from = to;
+    }
+    __syncthreads();
+    const int lo_bin = max(s.bin - 1, 0), hi_bin = s.bin + 1;
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h)
+      if (b0 + h >= lo_bin && b0 + h <= hi_bin) atomicAdd(&s.window, static_cast<int>(c[h]));
+    __syncthreads();
+    const bool fits = s.bin >= 0 && hi_bin < kBins - 1 && s.window <= kList;
+    if (!fits) {
+      cluster.sync();  // the histograms are read
+      return false;
+    }
+    const float from_here = static_cast<float>(lo_bin), past = hi_bin + 1.f;
+    unsigned long long above = 0, counted = 0;  // weights above the window, and of min_p or more
+    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
+      float top_of = v[0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) top_of = fmaxf(top_of, v[e]);
+      if (!(place_of(top_of) < past)) return;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float at = place_of(v[e]);
+        if (at < from_here) {
+          const float x = expf(scaled(v[e]));
+          const unsigned long long w = whole(x);
+          above += w;
+          if (x >= min_p) counted += w;
+        } else if (at < past) {
+          append(i + e, v[e]);
+        }
+      }
+    });
+    before_warp(warp_total(above), all);
+    if (tid == 0) s.above = all;
+    cluster.sync();
+    const unsigned long long over =
+        cluster_total(lane < ranks ? peer(lane)->above : 0ull, earlier);
+    const int n = gather();
+    cluster.sync();  // the lists are read
+    sort_descending(s.all, n);
+    unsigned long long lw[kPer], l_all;
+    running(n, lw, l_all);
+    if (!(static_cast<double>(over) < reach) || static_cast<double>(over + l_all) < reach) return false;
+    const int m = settle(n, lw, [&](int, unsigned long long before) {
+      return static_cast<double>(over + before) < reach;
+    });
+    for (int j = lane; j < m; j += 32) {
+      const int i = index_of(s.all[j]);
+      if (i < seg0 || i >= seg1) continue;
+      const float x = expf(scaled(value_of(s.all[j])));
+      if (x >= min_p) counted += whole(x);
+    }
+    mine = warp_total(counted);
+    return true;
+  };
+
   // Moves (edge, last) to token number `want` of the kept ones, or to the last of them whose
-  // weight before it is below p times the weight of all.
+  // weight before it is below p times the weight of all: for every row, with exact sums.
   auto cut = [&](bool by_weight, unsigned long long want) {
-    if (tid == 0) s.n_list = 0;
     boundary(by_weight, !by_weight, true, want, 0, 0, by_weight, bin_of);
     const int bin = s.bin;
     if (bin < 0) {  // fewer tokens than `want` (NaN is none): all stay, in every CTA alike
@@ -369,72 +685,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     const unsigned long long above_c = s.before_c, above_w = s.before_w;
     each([&](int i, float v) {
-      if (v == v && kept(i, v) && bin_of(v) == bin) {
-        const int at = atomicAdd(&s.n_list, 1);
-        if (at < kList) {
-          s.list_x[at] = v;
-          s.list_i[at] = i;
-        }
-      }
+      if (v == v && kept(i, v) && bin_of(v) == bin) append(i, v);
     });
     cluster.sync();
-    int first = lane < ranks ? peer(lane)->n_list : 0;
-    const int n = __reduce_add_sync(DDT_FULL_MASK, first);
+    const int n = gather();
+    cluster.sync();  // the lists are read
     if (n <= kList) {
-      // every CTA takes the whole list and finds the boundary by itself
-      for (int r = 0, at = 0; r < ranks; ++r) {
-        const Shared* o = peer(r);
-        const int m = __shfl_sync(DDT_FULL_MASK, first, r);
-        for (int j = tid; j < m; j += kThreads) {
-          const float v = o->list_x[j];
-          s.all_x[at + j] = v;
-          s.all_i[at + j] = o->list_i[j];
-          s.all_w[at + j] = by_weight ? weight(v) : 0ull;
-        }
-        at += m;
-      }
-      __syncthreads();
-      int kept_here = 0, order[kList / kThreads] = {};
-#pragma unroll
-      for (int h = 0; h < kList / kThreads; ++h) {
-        const int j = tid + h * kThreads;
-        order[h] = -1;
-        if (j < n) {
-          const float v = s.all_x[j];
-          const int i = s.all_i[j];
-          unsigned long long c = 0, w = 0;
-          for (int o = 0; o < n; ++o) {
-            const float vo = s.all_x[o];
-            if (vo > v || (vo == v && s.all_i[o] < i)) {
-              ++c;
-              w += s.all_w[o];
-            }
-          }
-          if (by_weight ? static_cast<double>(above_w + w) < reach : above_c + c < want) {
-            ++kept_here;
-            order[h] = static_cast<int>(c);
-          }
-        }
-      }
-      kept_here = __reduce_add_sync(DDT_FULL_MASK, kept_here);
-      if (lane == 0) s.warp_sum[0][warp] = kept_here;
-      __syncthreads();
-      int m = 0;
-      for (int w = 0; w < kWarps; ++w) m += static_cast<int>(s.warp_sum[0][w]);
-#pragma unroll
-      for (int h = 0; h < kList / kThreads; ++h)
-        if (order[h] == m - 1) {
-          s.edge = s.all_x[tid + h * kThreads];
-          s.last = s.all_i[tid + h * kThreads];
-        }
-      cluster.sync();  // the lists are read; (edge, last) is there
-      edge = s.edge;
-      last = s.last;
-      all_kept = false;
+      sort_descending(s.all, n);
+      unsigned long long w[kPer] = {}, all;
+      if (by_weight) running(n, w, all);
+      settle(n, w, [&](int j, unsigned long long before) {
+        return by_weight ? static_cast<double>(above_w + before) < reach : above_c + j < want;
+      });
       return;
     }
     // a long list: three steps over the bits of the key, from the top
-    cluster.sync();
     uint32_t prefix = 0;
     unsigned long long c_above = 0, w_above = 0, n_ties = 0;
     for (int level = 0; level < 3; ++level) {
@@ -470,18 +735,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     int mine = 0;
     each([&](int i, float v) { mine += v == value && kept(i, v); });
     mine = __reduce_add_sync(DDT_FULL_MASK, mine);
-    if (lane == 0) s.warp_sum[0][warp] = mine;
-    if (tid == 0) s.tie_index = V;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s.warp_sum[0][w];
-      all += s.warp_sum[0][w];
+    unsigned long long all, earlier;
+    unsigned long long before = before_warp(mine, all);
+    if (tid == 0) {
+      s.ties = static_cast<int>(all);
+      s.tie_index = V;
     }
-    if (tid == 0) s.ties = static_cast<int>(all);
     cluster.sync();
-    before += __reduce_add_sync(DDT_FULL_MASK, lane < rank ? peer(lane)->ties : 0);
-    long long left = static_cast<long long>(ties) - before;  // of this warp's
+    cluster_total(lane < ranks ? peer(lane)->ties : 0, earlier);
+    long long left = static_cast<long long>(ties - before - earlier);  // of this warp's
     if (left >= 1 && left <= mine) {
       for (int i0 = seg0; i0 < seg1; i0 += kStep) {
         const int i = i0 + lane * kVec;
@@ -513,6 +775,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     all_kept = false;
     cluster.sync();  // before the next search writes again
   };
+
+  unsigned long long mine = 0;  // kept weight of this warp's range
+  bool weighed = false;
   if (k == 1) {
     // the first of the largest
     int first = V;
@@ -520,12 +785,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     first = __reduce_min_sync(DDT_FULL_MASK, first);
     if (lane == 0) atomicMin(&s.tie_index, first);
     cluster.sync();
-    edge = top;
-    all_kept = false;
-    last = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
-  } else {
-    if (k < V) cut(false, k);
+    first = __reduce_min_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->tie_index : V);
+    if (rank == 0 && tid == 0) write(top, first, whole(1.f));
+    cluster.sync();
+    return;
+  }
+  if (k < V) {
+    if (by_list()) return;
+    cut(false, k);
     if (p < 1.0) cut(true, 0);
+  } else if (p < 1.0) {
+    weighed = nucleus(mine);
+    if (!weighed) cut(true, 0);
   }
 
   // ---- 3. kept weight, target, token ---------------------------------------------------------
@@ -536,6 +807,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     hi = in ? hi : 0;
     lo = in ? lo : 0;
   };
+  const bool plain = all_kept && min_p <= 0.f;  // every token counts
   // kept weight of the warp's [begin, end)
   auto weigh = [&](int begin, int end) {
     unsigned long long sum = 0;
@@ -546,7 +818,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) any |= v[e] >= edge;
       }
-      if (any) {
+      if (plain) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          uint32_t h, l;
+          limbs(expf(scaled(v[e])), h, l);
+          hi += h;
+          lo += l;
+        }
+      } else if (any) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
           uint32_t h, l;
@@ -557,41 +837,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       }
       sum += (static_cast<unsigned long long>(hi) << 20) + lo;
     });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(DDT_FULL_MASK, sum, o);
-    return sum;
+    return warp_total(sum);
   };
-  // weight before this warp's part, of the parts of the CTA's warps in order
-  auto before_warp = [&](unsigned long long part, unsigned long long& all) {
-    __syncthreads();
-    if (lane == 0) s.warp_sum[0][warp] = part;
-    __syncthreads();
-    unsigned long long before = 0;
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const unsigned long long o = s.warp_sum[0][w];
-      if (w < warp) before += o;
-      all += o;
-    }
-    return before;
-  };
-  unsigned long long mine = weigh(seg0, seg1), all;
+  unsigned long long all, earlier;
+  if (!weighed) mine = weigh(seg0, seg1);
   unsigned long long before = before_warp(mine, all);
   if (tid == 0) s.sum = all;
   cluster.sync();
-  unsigned long long total = lane < ranks ? peer(lane)->sum : 0ull;
-  unsigned long long earlier = lane < rank ? total : 0ull;
-#pragma unroll
-  for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(DDT_FULL_MASK, total, o);
-    earlier += __shfl_xor_sync(DDT_FULL_MASK, earlier, o);
-  }
-  total = __shfl_sync(DDT_FULL_MASK, total, 0);
-  earlier = __shfl_sync(DDT_FULL_MASK, earlier, 0);
-  long long t = static_cast<long long>(floor(static_cast<double>(a.u[row]) * static_cast<double>(total)));
-  t = max(min(t, static_cast<long long>(total) - 1), 0ll);
-  unsigned long long target = static_cast<unsigned long long>(t);
+  const unsigned long long total =
+      cluster_total(lane < ranks ? peer(lane)->sum : 0ull, earlier);
+  // the last look at another CTA's shared memory: those without the token leave once all have
+  // had theirs
+  cluster.barrier_arrive();
+  unsigned long long target = target_of(total);
   if (earlier <= target && target < earlier + all) {  // this CTA holds the token
     // its warps share the range of the warp that holds it, until a warp's part is one step
     target -= earlier;
@@ -641,14 +899,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
           }
           at += w[e];
         }
-        a.tokens[row] = pick;
-        if (a.logprobs)
-          a.logprobs[row] = static_cast<float>(static_cast<double>(scaled(value)) -
-                                               (log(static_cast<double>(total)) - kLogUnit));
+        write(value, pick, total);
       }
     }
   }
-  cluster.sync();  // no CTA leaves while another may read its shared memory
+  cluster.barrier_wait();
 }
 
 }  // namespace sample
