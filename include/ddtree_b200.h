@@ -532,8 +532,9 @@ int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
  * the weight of all of these (at least one); of these the ones with exp(z_i) >= min_p (at most
  * 1).  tokens[r] (i64) is the first token by index whose running kept weight exceeds floor(u *
  * total); logprobs[r] (f32, may be NULL) the log of its share of the kept weight.  temperature <
- * 1e-5 keeps the first token alone.  NaN logits count as -inf; -inf tokens are never drawn; a row
- * with no other gives token -1 and logprob -inf.  vocab < 2^22.
+ * 1e-5 keeps the first token alone; one above 1e30 counts as 1e30.  NaN logits count as -inf;
+ * -inf tokens are never drawn; a row with no other gives token -1 and logprob -inf.
+ * vocab < 2^22.
  * Replaces sample() at temperature > 0 (model/utils.py:28-35: softmax and torch.multinomial).
  * No workspace. */
 int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
