@@ -804,19 +804,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     hi = in ? hi : 0;
     lo = in ? lo : 0;
   };
-  const bool plain = all_kept && min_p <= 0.f;  // every token counts
   // kept weight of the warp's [begin, end)
   auto weigh = [&](int begin, int end) {
     unsigned long long sum = 0;
-    if (plain) {
+    if (all_kept) {
       vectors(begin, end, [&](int, float (&v)[kVec]) {
         uint32_t hi = 0, lo = 0;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
+          const float x = expf(scaled(v[e]));
           uint32_t h, l;
-          limbs(expf(scaled(v[e])), h, l);
-          hi += h;
-          lo += l;
+          limbs(x, h, l);
+          if (x >= min_p) {
+            hi += h;
+            lo += l;
+          }
         }
         sum += (static_cast<unsigned long long>(hi) << 20) + lo;
       });
@@ -925,10 +927,11 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   sample::Args a{logits, static_cast<int>(vocab), row_stride, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs, aligned(logits, 16) && (row_stride * size) % 16 == 0};
   // as many CTAs per row as keep the rows in one wave (two CTAs per SM), or the rows in flight
-  // in half of L2 (they are read again), and no more than leave each thread one load
+  // in L2 (they are read again; 257 rows of 608 KB: 83 us with 2 CTAs each, 95 with 4), and no
+  // more than leave each thread one load
   int ranks = 1;
   while (ranks < sample::kMaxCluster && vocab > ranks * sample::kThreads * (16 / size) &&
-         (rows * ranks * 2 <= 2 * 148 || 2 * 148 / ranks * vocab * size > (int64_t(64) << 20)))
+         (rows * ranks * 2 <= 2 * 148 || 2 * 148 / ranks * vocab * size > (int64_t(100) << 20)))
     ranks *= 2;
   auto kernel = dtype == DDT_BF16 ? sample::sample_kernel<true> : sample::sample_kernel<false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
