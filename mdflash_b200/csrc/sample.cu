@@ -237,24 +237,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       }
     }
   };
-  // f(first index, kVec values) over [begin, end) of this warp: kBatch loads are in flight
-  // before the first is used
-  auto vectors = [&](int begin, int end, auto f) DDT_INLINE {
+  // f(first index, kVec values) over [begin, end) of this warp, every `every`-th step of it:
+  // kBatch loads are in flight before the first is used
+  auto vectors = [&](int begin, int end, int every, auto f) DDT_INLINE {
     constexpr int kBatch = 4;
+    const int step = kStep * every;
     int i = begin + lane * kVec;
     if (a.vectors)
-      for (; i - lane * kVec + kBatch * kStep <= end; i += kBatch * kStep) {
+      for (; i - lane * kVec + (kBatch - 1) * step + kStep <= end; i += kBatch * step) {
         uint4 r[kBatch];
 #pragma unroll
-        for (int h = 0; h < kBatch; ++h) r[h] = vec_at(i + h * kStep);
+        for (int h = 0; h < kBatch; ++h) r[h] = vec_at(i + h * step);
 #pragma unroll
         for (int h = 0; h < kBatch; ++h) {
           float v[kVec];
           spread(r[h], v);
-          f(i + h * kStep, v);
+          f(i + h * step, v);
         }
       }
-    for (; i < end; i += kStep) {
+    for (; i < end; i += step) {
       float v[kVec];
       load(i, end, v);
       f(i, v);
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   };
   // f(index, value) over this warp's range
   auto each = [&](auto f) DDT_INLINE {
-    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
+    vectors(seg0, seg1, 1, [&](int i, float (&v)[kVec]) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(i + e, v[e]);
     });
@@ -377,6 +378,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     return static_cast<int>(__float_as_uint(__fadd_rz(fminf(place_of(v), kBins - 1.f), 8388608.f)) -
                             0x4b000000u);
   };
+  // Where a search only has to come close (its result is checked), a quarter of the row is
+  // counted: the counters' updates, several to one bank, are what a counting pass waits for.
+  const int every = per_warp >= 8 * kStep ? 4 : 1;
   auto clear = [&] {
     for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
     if (tid == 0) {
@@ -385,12 +389,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     __syncthreads();
   };
-  // counts of this thread's kOwn bins b0 .. over the cluster
-  auto bin_counts = [&](int b0, unsigned long long (&c)[kOwn]) {
-    for (int r = 0; r < ranks; ++r) {
-      const uint4 o = *reinterpret_cast<const uint4*>(&peer(r)->count[b0]);
-      c[0] += o.x, c[1] += o.y, c[2] += o.z, c[3] += o.w;
+  // this thread's kOwn bins b0 .. of every CTA of the cluster, all loads in flight together (one
+  // after the other eight of them took 5 us)
+  auto bins_of_all = [&](const uint32_t* own, int b0, auto add) {
+    uint4 o[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      o[r] = r < ranks ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(own, r) + b0)
+                       : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      add(0, o[r].x);
+      add(1, o[r].y);
+      add(2, o[r].z);
+      add(3, o[r].w);
     }
+  };
+  auto bin_counts = [&](int b0, unsigned long long (&c)[kOwn]) {
+    bins_of_all(s.count, b0, [&](int h, uint32_t x) { c[h] += x; });
   };
   // Histogram of the kept tokens by `bin` (those with a bin >= 0), added over the cluster; then
   // the bin that holds the boundary: by weight the last one whose weight before it is below
@@ -419,16 +435,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     unsigned long long c[kOwn] = {}, w[kOwn] = {}, c_sum = 0, w_sum = 0;
     const int b0 = (ascending ? tid : kThreads - 1 - tid) * kOwn;
     if (count) bin_counts(b0, c);
-    if (by_weight)
-      for (int r = 0; r < ranks; ++r) {
-        const Shared* o = peer(r);
-        const uint4 ol = *reinterpret_cast<const uint4*>(&o->lo[b0]),
-                    oh = *reinterpret_cast<const uint4*>(&o->hi[b0]);
-        w[0] += (static_cast<unsigned long long>(oh.x) << 32) + ol.x;
-        w[1] += (static_cast<unsigned long long>(oh.y) << 32) + ol.y;
-        w[2] += (static_cast<unsigned long long>(oh.z) << 32) + ol.z;
-        w[3] += (static_cast<unsigned long long>(oh.w) << 32) + ol.w;
-      }
+    if (by_weight) {
+      bins_of_all(s.lo, b0, [&](int h, uint32_t x) { w[h] += x; });
+      bins_of_all(s.hi, b0, [&](int h, uint32_t x) { w[h] += static_cast<unsigned long long>(x) << 32; });
+    }
 #pragma unroll
     for (int h = 0; h < kOwn; ++h) {
       c_sum += c[h];
@@ -466,12 +476,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     const int mine = lane < ranks ? peer(lane)->n_list : 0;
     const int n = __reduce_add_sync(DDT_FULL_MASK, mine);
     if (n > kList) return n;
-    for (int r = 0, at = 0; r < ranks; ++r) {
-      const unsigned long long* o = peer(r)->list;
-      const int m = __shfl_sync(DDT_FULL_MASK, mine, r);
-      for (int j = tid; j < m; j += kThreads) s.all[at + j] = o[j];
-      at += m;
+    int length[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) length[r] = __shfl_sync(DDT_FULL_MASK, mine, r);
+    unsigned long long t[kPer];  // loaded from all CTAs at once
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      int j = tid + h * kThreads, from = 0;
+      if (j >= n) continue;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster - 1; ++r)
+        if (from == r && j >= length[r]) {
+          j -= length[r];
+          ++from;
+        }
+      t[h] = peer(from)->list[j];
     }
+#pragma unroll
+    for (int h = 0; h < kPer; ++h)
+      if (tid + h * kThreads < n) s.all[tid + h * kThreads] = t[h];
     __syncthreads();
     return n;
   };
@@ -510,18 +533,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   };
 
   // top-k on a list of all candidates, by the first CTA: false, and nothing done, where the
-  // list would be too long.
+  // list would be too long, or turns out too long or too short.
   auto by_list = [&]() -> bool {
-    boundary(false, true, true, k, 0, 0, false, bin_of);
-    const int bin = s.bin;
-    // (without a bin there are fewer tokens than k, NaN being none)
-    const bool fits = bin >= 0 && s.before_c + s.bin_c <= kList;
-    if (!fits) {
-      cluster.sync();  // the histograms are read
-      return false;
+    clear();
+    vectors(seg0, seg1, every, [&](int, float (&v)[kVec]) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (v[e] == v[e]) atomicAdd(&s.count[bin_of(v[e])], 1u);
+    });
+    cluster.sync();
+    unsigned long long c[kOwn] = {}, c_sum = 0, c0, w0, w_all;
+    bin_counts(tid * kOwn, c);
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) c_sum += c[h];
+    scan2(c_sum, 0ull, s, c0, w0, w_all);
+    // half as many again as k, and some: a count of a quarter is off by a few square roots
+    const unsigned long long want = (k + k / 2 + 64) / every;
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+      if (c0 < want && want <= c0 + c[h]) {
+        s.bin = tid * kOwn + h;
+        s.window = static_cast<int>(min(c0 + c[h], 1ull << 20)) * every;
+      }
+      c0 += c[h];
     }
+    __syncthreads();
+    const int bin = s.bin < 0 ? kBins - 1 : s.bin;  // (none: the row has not that many)
+    const bool fits = s.bin < 0 ? V <= kList : s.window <= kList;
+    cluster.sync();  // the histograms are read
+    if (!fits) return false;
     const float past = bin + 1.f;
-    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
+    vectors(seg0, seg1, 1, [&](int i, float (&v)[kVec]) {
       float top_of = v[0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) top_of = fmaxf(top_of, v[e]);
@@ -531,9 +573,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         if (place_of(v[e]) < past) append(i + e, v[e]);
     });
     cluster.sync();
-    const int listed = rank == 0 ? gather() : 0;
+    const int listed = __reduce_add_sync(DDT_FULL_MASK, lane < ranks ? peer(lane)->n_list : 0);
+    const bool good = listed >= k && listed <= kList;
+    if (good && rank == 0) gather();
     cluster.sync();  // the lists are read
-    if (rank != 0) return true;
+    if (!good || rank != 0) return good;
     sort_descending(s.all, listed);
     const int n = min(listed, k);
     unsigned long long w[kPer], all;
@@ -551,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     __syncthreads();
     sort_descending(s.list, n);
-    unsigned long long own[kPer], sum = 0, c0, before, total;
+    unsigned long long own[kPer], sum = 0, before, total;
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
       const int j = tid * kPer + h;
@@ -578,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   auto nucleus = [&](unsigned long long& mine) -> bool {
     clear();
     unsigned long long sum = 0, all, earlier;
-    vectors(seg0, seg1, [&](int, float (&v)[kVec]) {
+    vectors(seg0, seg1, 1, [&](int, float (&v)[kVec]) {
       uint32_t hi = 0, lo = 0;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
@@ -606,30 +650,48 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       c_sum += c[h];
       w_sum += w[h];
     }
+    if (tid == 0) {
+      s.range0 = kBins;
+      s.range1 = -1;
+    }
     scan2(c_sum, w_sum, s, c0, w0, w_all);
     // judged from the row's end: what follows the boundary is many light tokens, whose
     // distances from their intervals' middles cancel; a heavy token's would not
     double from = static_cast<double>(whole_row) - static_cast<double>(w_all - w0);
+    unsigned long long at = c0;
 #pragma unroll
     for (int h = 0; h < kOwn; ++h) {
       const double to = from + static_cast<double>(w[h]);
-      if (from < reach && !(to < reach)) s.bin = b0 + h;
+      if (from < reach && !(to < reach)) {
+        s.bin = b0 + h;
+        s.before_c = at;
+      }
       from = to;
+      at += c[h];
     }
     __syncthreads();
-    const int lo_bin = max(s.bin - 1, 0), hi_bin = s.bin + 1;
+    // and its neighbours: one interval on either side, and more where they hold few tokens (the
+    // list is sorted: 1500 tokens instead of 800 cost 14 us of 45)
+    const long long near = static_cast<long long>(s.before_c), room = 128;
+    at = c0;
 #pragma unroll
-    for (int h = 0; h < kOwn; ++h)
-      if (b0 + h >= lo_bin && b0 + h <= hi_bin) atomicAdd(&s.window, static_cast<int>(c[h]));
-    __syncthreads();
-    const bool fits = s.bin >= 0 && hi_bin < kBins - 1 && s.window <= kList;
-    if (!fits) {
-      cluster.sync();  // the histograms are read
-      return false;
+    for (int h = 0; h < kOwn; ++h) {
+      const int b = b0 + h;
+      if (b <= s.bin && (b >= s.bin - 1 || static_cast<long long>(at) >= near - room))
+        atomicMin(&s.range0, b);
+      at += c[h];
+      if (s.bin >= 0 && b >= s.bin && (b <= s.bin + 1 || static_cast<long long>(at) <= near + room))
+        atomicMax(&s.range1, b);
+      if (b >= s.bin - 1 && b <= s.bin + 1) atomicAdd(&s.window, static_cast<int>(c[h]));
     }
+    __syncthreads();
+    const int lo_bin = s.range0, hi_bin = s.range1;
+    const bool fits = s.bin >= 0 && s.window <= kList - 2 * room;
+    cluster.sync();  // the histograms are read
+    if (!fits) return false;
     const float from_here = static_cast<float>(lo_bin), past = hi_bin + 1.f;
     unsigned long long above = 0, counted = 0;  // weights above the window, and of min_p or more
-    vectors(seg0, seg1, [&](int i, float (&v)[kVec]) {
+    vectors(seg0, seg1, 1, [&](int i, float (&v)[kVec]) {
       float top_of = v[0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) top_of = fmaxf(top_of, v[e]);
@@ -654,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         cluster_total(lane < ranks ? peer(lane)->above : 0ull, earlier);
     const int n = gather();
     cluster.sync();  // the lists are read
+    if (n > kList) return false;
     sort_descending(s.all, n);
     unsigned long long lw[kPer], l_all;
     running(n, lw, l_all);
@@ -808,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   auto weigh = [&](int begin, int end) {
     unsigned long long sum = 0;
     if (all_kept) {
-      vectors(begin, end, [&](int, float (&v)[kVec]) {
+      vectors(begin, end, 1, [&](int, float (&v)[kVec]) {
         uint32_t hi = 0, lo = 0;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
@@ -823,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         sum += (static_cast<unsigned long long>(hi) << 20) + lo;
       });
     } else {
-      vectors(begin, end, [&](int i, float (&v)[kVec]) {
+      vectors(begin, end, 1, [&](int i, float (&v)[kVec]) {
         float top_of = v[0];
 #pragma unroll
         for (int e = 1; e < kVec; ++e) top_of = fmaxf(top_of, v[e]);
