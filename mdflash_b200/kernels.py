@@ -3,6 +3,7 @@ the current CUDA stream of the tensors' device and never synchronise the host.""
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 from dataclasses import dataclass
 
@@ -875,11 +876,11 @@ class PageStep:
 
     @staticmethod
     def allocate(device, n_requests: int, max_tokens: int) -> "PageStep":
-        i32 = dict(dtype=torch.int32, device=device)
-        i64 = dict(dtype=torch.int64, device=device)
-        return PageStep(torch.empty(n_requests, **i32), torch.empty(n_requests + 1, **i32),
-                        torch.empty(max_tokens, **i64), torch.empty(max_tokens, **i64),
-                        torch.empty(1, **i32))
+        lens, cu_new, count = torch.empty(2 * n_requests + 2, dtype=torch.int32, device=device) \
+            .split_with_sizes([n_requests, n_requests + 1, 1])
+        slots, positions = torch.empty(2 * max_tokens, dtype=torch.int64, device=device) \
+            .split_with_sizes([max_tokens, max_tokens])
+        return PageStep(lens, cu_new, slots, positions, count)
 
 
 # These launches are short next to their host side, so its checks are kept to one call per
@@ -899,6 +900,15 @@ def _device_of(*ts: torch.Tensor) -> int:
 def _need(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
+
+
+@functools.cache
+def _paged_bytes() -> tuple[int, int]:
+    """Workspace bytes of ddt_page_tables and ddt_paged_attn, the same for all sizes up to the
+    compiled limits."""
+    lib = _lib.load()
+    return (lib.ddt_page_tables_workspace_bytes(_lib.DDT_MAX_PAGED_REQUESTS),
+            lib.ddt_paged_attn_workspace_bytes(1 << 20, 1 << 20, 64, 1))
 
 
 def _table_view(block_table: torch.Tensor, requests: int) -> tuple[int, int]:
@@ -941,7 +951,7 @@ def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     if status is None:
         status = attention_status(old_lens.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(old_lens.device, "page_tables", lib.ddt_page_tables_workspace_bytes(R))
+    ws = WORKSPACES.get(old_lens.device, "page_tables", _paged_bytes()[0])
     check(lib.ddt_page_tables(
         old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(), t_stride, cols,
         page_size, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
@@ -989,7 +999,7 @@ def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torc
             not slot_map.is_contiguous():
         raise ValueError("slot_map must be contiguous i64 with a slot per token")
     if out is None:
-        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=qkv.device)
+        out = qkv.new_empty((T, hq, d))
     else:
         _need(out, torch.bfloat16, (T, hq, d), "out")
         _device_of(qkv, out)
@@ -1024,7 +1034,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _need(cu_new, torch.int32, (R + 1,), "cu_new")
     t_stride, cols = _table_view(block_table, R)
     if out is None:
-        out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((T, hq, d))
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
             out.get_device() != idx:
         raise ValueError("out must be like q")
@@ -1032,8 +1042,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if status is None:
         status = attention_status(q.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(q.device, "paged_attn",
-                        lib.ddt_paged_attn_workspace_bytes(T, max_new, hq, hkv))
+    ws = WORKSPACES.get(q.device, "paged_attn", _paged_bytes()[1])
     check(lib.ddt_paged_attn(
         q.data_ptr(), q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
         ps, sp, sh, sr, block_table.data_ptr(), t_stride, cols, cu_new.data_ptr(),
@@ -1066,12 +1075,12 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
             _need(t, dt, (rows,), name)
         rules.append(None if t is None else t.data_ptr())
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        out = u.new_empty(rows, dtype=torch.int64)
     else:
         _device_of(logits, out)
         _need(out, torch.int64, (rows,), "out")
     if logprobs is None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        logprobs = u.new_empty(rows)
     else:
         _device_of(logits, logprobs)
         _need(logprobs, torch.float32, (rows,), "logprobs")
