@@ -454,7 +454,8 @@ int ddt_mask_to_bits(const void* mask, int dtype, int64_t n_nodes, int64_t row_s
  * One pool of pages serves many requests: k_pages / v_pages hold n_pages pages of page_size
  * rows per KV head, element (page, head, row, d) at page * page_stride + head * head_stride +
  * row * row_stride + d (elements; the same strides for K and V; both [page, head, row] and
- * [page, row, head] orders are strides).  page_size is a power of two from 16 to 1024.
+ * [page, row, head] orders are strides).  page_size is a power of two from 16 to 1024,
+ * max_pages * page_size at most 2^30.
  * block_table i32 [n_requests, max_pages] (row stride table_stride): entry j of request r is the page of its rows
  * [j * page_size, (j + 1) * page_size).  A slot is page * page_size + row.  Lengths, offsets
  * and tables live on the device, so a recorded step serves every length.  No counterpart in

@@ -774,7 +774,7 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   if (head_dim != kHeadDim || q_heads / kv_heads > kMaxGroup) return DDT_ERR_CAPACITY;
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return DDT_ERR_CAPACITY;
   if (n_requests > DDT_MAX_PAGED_REQUESTS || n_tokens > 0x7fffffff || n_pages >= 0x7fffffff ||
-      max_pages > 0x7fffffff / page_size || kv_heads > 65535)
+      max_pages > (int64_t(1) << 30) / page_size || kv_heads > 65535)
     return DDT_ERR_CAPACITY;
   if (n_tokens == 0 || max_new == 0) return DDT_OK;
   if (!q || !k_pages || !v_pages || !block_table || !cu_new || !kv_lens || !out)

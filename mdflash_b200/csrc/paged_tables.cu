@@ -238,7 +238,7 @@ extern "C" int ddt_page_tables(const int32_t* old_lens, const int32_t* new_lens,
     return DDT_ERR_INVALID;
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return DDT_ERR_CAPACITY;
   if (n_requests > DDT_MAX_PAGED_REQUESTS || max_tokens > 0x7fffffff || free_capacity > 0x7fffffff ||
-      max_pages * page_size > 0x7fffffff)
+      max_pages > (int64_t(1) << 30) / page_size)
     return DDT_ERR_CAPACITY;
   if (!workspace || workspace_bytes < sizeof(unsigned int)) return DDT_ERR_WORKSPACE;
   if (!aligned(workspace, 4)) return DDT_ERR_ALIGN;

@@ -324,6 +324,9 @@ ATTN = {
     "chunk_among_decodes": ([900, 5000, 64, 1, 777], [1, 400, 1, 1, 1], 16, 8, 16),
     "chunk_page_512": ([1500, 513], [512, 100], 8, 8, 512),
     "many_requests": (list(range(1, 301)), [1] * 300, 8, 2, 16),
+    # both kernels: a chunk, single tokens, idle places and a request of 20 rows between them
+    "chunk_among_30": ([37 * i + 1 for i in range(15)] + [700, 0, 64] + [50 * i + 9 for i in range(13)],
+                       [1] * 15 + [300, 0, 10] + [1] * 13, 16, 8, 16),
 }
 
 
@@ -425,6 +428,25 @@ def test_paged_attention_far_pages(cuda_device):
     out = c.run()
     assert torch.equal(out, near)
     c.check(out)
+
+
+def test_paged_attention_mixed_batch_recorded(cuda_device):
+    """Both kernels and the merge in a recorded graph, on a side stream, replayed back to back."""
+    lens, news, hq, hkv, page = ATTN["chunk_among_30"]
+    c = _Case(cuda_device, lens, news, hq, hkv, page, seed=2)
+    eager = c.run()
+    c.check(eager)
+    outs = [torch.zeros_like(c.q) for _ in range(4)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for o in outs:
+            c.run(out=o)
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, eager) for o in outs)
 
 
 @pytest.mark.parametrize("news", [[1, 1, 1, 1], [16, 3, 16, 1], [100, 1, 300, 64]])

@@ -104,6 +104,39 @@ def test_sample_full_vocabulary(cuda_device, only, dtype):
     _check(cuda_device, x.to(cuda_device), u, temp, k, p, mp)
 
 
+@pytest.mark.parametrize("p", [0.05, 0.5, 0.9, 0.95, 0.9999])
+@pytest.mark.parametrize("spread,heavy", [(0.3, 0), (3.0, 0), (3.0, 8), (8.0, 3), (0.01, 0)])
+def test_sample_nucleus_boundaries(cuda_device, p, spread, heavy):
+    """top-p alone over rows from flat (the nucleus is most of the vocabulary) to spiky (a few
+    tokens), where the boundary is first judged by intervals of the logits; temperatures whose
+    quotients are awkward (significands of all ones)."""
+    rng = np.random.default_rng(int(p * 1e4) + heavy)
+    rows, V = 4, 60001
+    x = rng.standard_normal((rows, V)).astype(np.float32) * spread
+    for r in range(rows):
+        x[r, rng.integers(0, V, heavy)] += rng.random(heavy).astype(np.float32) * 12
+    u = [float(np.float32(v)) for v in rng.random(rows)]
+    temp = [1.0, float(np.nextafter(np.float32(1), np.float32(0))), 0.7,
+            float(np.nextafter(np.float32(2), np.float32(0)))]
+    mp = [0.0, 0.0, 0.001, 0.2]
+    for dtype in (torch.float32, torch.bfloat16):
+        _check(cuda_device, torch.from_numpy(x).to(dtype).to(cuda_device), u, temp, None, [p] * rows, mp)
+
+
+@pytest.mark.parametrize("k", [1200, 1300, 2047, 5000, 59999])
+def test_sample_long_candidate_lists(cuda_device, k):
+    """top-k around and beyond what one list holds, with and without top-p, NaN in the row."""
+    rng = np.random.default_rng(k)
+    rows, V = 3, 60001
+    x = rng.standard_normal((rows, V)).astype(np.float32) * 2
+    x[1, ::3] = np.nan
+    x[2, 100:59000] = -np.inf
+    u = [float(np.float32(v)) for v in rng.random(rows)]
+    for p in (1.0, 0.97):
+        _check(cuda_device, torch.from_numpy(x).to(cuda_device), u, [0.9] * rows, [k] * rows,
+               [p] * rows, [0.0] * rows)
+
+
 def test_sample_ties(cuda_device):
     """Rows of a few distinct values: cuts fall inside long runs of equal logits, which are
     kept from the lowest index."""
