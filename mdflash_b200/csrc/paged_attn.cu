@@ -28,7 +28,7 @@
 // TMEM columns: S0/P0 [0,128) O0 [128,256) S1/P1 [256,384) O1 [384,512).
 // Every wait is bounded; a timeout sets *status and unwinds the CTA.
 //
-// Measured, four chunks of 2048 tokens at the end of 2.5k to 10k keys, 32 query heads over 8
+// Measured, four chunks of up to 2048 tokens over 3k to 9.5k keys, 32 query heads over 8
 // (452 GFLOP): 380 us or 1190 TFLOP/s, 0.72 of the measured bf16 burst; 448 us in a loop of
 // seconds, where the power limit lowers the clock.  The tensor pipe is active in 65% of the
 // cycles; the bound is one query tile's chain per key tile (TMEM read, maximum, exponentials,

@@ -22,8 +22,8 @@
 // CTAs exchange values through distributed shared memory, with one cluster barrier each time.
 //
 // Measured over 151936 logits: one fp32 row with top-k 50 and top-p 0.95 18 us, with top-p alone
-// 31 us, untruncated 12 us (all latency: passes of 3 to 8 us, barriers and remote reads between
-// them); 64 bf16 rows of mixed rules 56 us (the slowest row); 257 fp32 rows untruncated 83 us,
+// 30 us, untruncated 12 us (all latency: passes of 3 to 8 us, barriers and remote reads between
+// them); 64 bf16 rows of mixed rules 55 us (the slowest row); 257 fp32 rows untruncated 83 us,
 // 1.9 TB/s: the exponential, its quotient and the split into whole numbers are 25 instructions
 // per logit, and rows in step read HBM and compute in turn.
 #include <cooperative_groups.h>
@@ -118,43 +118,6 @@ __device__ __forceinline__ int index_of(unsigned long long t) {
   return static_cast<int>(~static_cast<uint32_t>(t));
 }
 
-// Sort of n <= kList numbers in descending order by the whole block.  Up to kRanked of them by
-// counting the larger ones (n steps without a barrier: 140 numbers in 0.4 us, against 36
-// barriers), more by a bitonic sort, whose places from n to the next power of two become 0.
-constexpr int kRanked = 256;
-static_assert(kRanked <= kThreads, "one number per thread");
-__device__ __forceinline__ void sort_descending(unsigned long long* a, int n) {
-  if (n <= kRanked) {
-    const int t = threadIdx.x;
-    const unsigned long long x = t < n ? a[t] : 0ull;
-    int rank = 0;
-    if (t < n) {
-#pragma unroll 8
-      for (int o = 0; o < n; ++o) rank += a[o] > x || (a[o] == x && o < t);
-    }
-    __syncthreads();
-    if (t < n) a[rank] = x;
-    __syncthreads();
-    return;
-  }
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int j = n + threadIdx.x; j < size; j += kThreads) a[j] = 0ull;
-  __syncthreads();
-  for (int run = 2; run <= size; run <<= 1)
-    for (int d = run >> 1; d > 0; d >>= 1) {
-      for (int t = threadIdx.x; t < size >> 1; t += kThreads) {
-        const int i = 2 * t - (t & (d - 1)), j = i + d;
-        const unsigned long long x = a[i], y = a[j];
-        if ((x < y) == ((i & run) == 0)) {
-          a[i] = y;
-          a[j] = x;
-        }
-      }
-      __syncthreads();
-    }
-}
-
 // Exclusive block scan of (c, w) in thread order; returns the totals too.
 __device__ __forceinline__ void scan2(unsigned long long c, unsigned long long w, Shared& s,
                                       unsigned long long& c_before, unsigned long long& w_before,
@@ -188,6 +151,68 @@ __device__ __forceinline__ void scan2(unsigned long long c, unsigned long long w
     }
     w_all += b;
   }
+}
+
+// Sort of n <= kList numbers `a` in descending order by the whole block; zeros are dropped, and
+// the number of the others is returned.  `bin` maps a number to an interval in [0, kBins), no
+// larger number to a higher one.  Up to kRanked numbers by counting the larger ones of each (140
+// numbers in 0.4 us).  More by the intervals: a count, the prefix of the counts, every number to
+// its interval's part of `scratch` [kList], and counting within the part (1400 numbers in about
+// 3 us; a bitonic sort's 66 barriers took 25).
+constexpr int kRanked = 256;
+static_assert(kRanked <= kThreads, "one number per thread");
+template <typename Bin>
+__device__ __forceinline__ int sort_descending(unsigned long long* a, int n,
+                                               unsigned long long* scratch, Shared& s, Bin bin) {
+  const int tid = threadIdx.x;
+  if (n <= kRanked) {
+    const unsigned long long x = tid < n ? a[tid] : 0ull;
+    int rank = 0;
+    if (x) {
+#pragma unroll 8
+      for (int o = 0; o < n; ++o) rank += a[o] > x;
+    }
+    const int m = __syncthreads_count(x != 0);
+    if (x) a[rank] = x;
+    __syncthreads();
+    return m;
+  }
+  for (int b = tid; b < kBins; b += kThreads) s.count[b] = 0;
+  __syncthreads();
+  unsigned long long x[kPer], before, w0, w_all;
+  int b[kPer], at[kPer];
+#pragma unroll
+  for (int h = 0; h < kPer; ++h) {
+    const int j = tid + h * kThreads;
+    x[h] = j < n ? a[j] : 0ull;
+    if (x[h]) {
+      b[h] = bin(x[h]);
+      at[h] = atomicAdd(&s.count[b[h]], 1u);
+    }
+  }
+  __syncthreads();
+  const uint4 c = *reinterpret_cast<const uint4*>(&s.count[tid * kOwn]);
+  static_assert(kOwn == 4, "one load per thread");
+  scan2(static_cast<unsigned long long>(c.x) + c.y + c.z + c.w, c.x + c.y + c.z + c.w, s, before, w0,
+        w_all);
+  const uint32_t f = static_cast<uint32_t>(before);
+  *reinterpret_cast<uint4*>(&s.lo[tid * kOwn]) =
+      make_uint4(f, f + c.x, f + c.x + c.y, f + c.x + c.y + c.z);
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < kPer; ++h)
+    if (x[h]) scratch[s.lo[b[h]] + at[h]] = x[h];
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < kPer; ++h) {
+    if (!x[h]) continue;
+    const uint32_t from = s.lo[b[h]], to = from + s.count[b[h]];
+    uint32_t rank = from;
+    for (uint32_t o = from; o < to; ++o) rank += scratch[o] > x[h];
+    a[rank] = x[h];
+  }
+  __syncthreads();
+  return static_cast<int>(w_all);
 }
 
 template <bool kBF16>
@@ -403,6 +428,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   // Where a search only has to come close (its result is checked), a quarter of the row is
   // counted: the counters' updates, several to one bank, are what a counting pass waits for.
   const int every = per_warp >= 8 * kStep ? 4 : 1;
+  // interval of a listed token among kBins that share the intervals [b0, b1] of the row
+  auto list_bin = [&](int b0, int b1) {
+    const float scale = (kBins - 1.f) / (b1 + 1 - b0);
+    return [&, b0, scale](unsigned long long t) {
+      const float at = (place_of(value_of(t)) - b0) * scale;
+      return __float2int_rz(fminf(fmaxf(at, 0.f), kBins - 1.f));
+    };
+  };
   auto clear = [&] {
     for (int b = tid; b < kBins; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
     if (tid == 0) {
@@ -600,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     if (good && rank == 0) gather();
     cluster.sync();  // the lists are read
     if (!good || rank != 0) return good;
-    sort_descending(s.all, listed);
+    sort_descending(s.all, listed, s.list, s, list_bin(0, bin));
     const int n = min(listed, k);
     unsigned long long w[kPer], all;
     running(n, w, all);
@@ -616,13 +649,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
       s.list[j] = in ? (t << 32) | (t >> 32) : 0ull;
     }
     __syncthreads();
-    sort_descending(s.list, n);
+    // (intervals of equal runs of indices)
+    const int run = max(32 - __clz(V - 1) - 11, 0);
+    const int m = sort_descending(s.list, n, s.all, s, [&](unsigned long long t) {
+      return static_cast<int>(~static_cast<uint32_t>(t >> 32) >> run);
+    });
     unsigned long long own[kPer], sum = 0, before, total;
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
       const int j = tid * kPer + h;
-      const unsigned long long t = j < n ? s.list[j] : 0ull;
-      own[h] = t ? weight(key_f32(static_cast<uint32_t>(t))) : 0ull;
+      own[h] = j < m ? weight(key_f32(static_cast<uint32_t>(s.list[j]))) : 0ull;
       sum += own[h];
     }
     scan2(0ull, sum, s, c0, before, total);
@@ -693,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
     __syncthreads();
     // and its neighbours: one interval on either side, and more where they hold few tokens (the
-    // list is sorted: 1500 tokens instead of 800 cost 14 us of 45)
+    // list is sorted)
     const long long near = static_cast<long long>(s.before_c), room = 128;
     at = c0;
 #pragma unroll
@@ -739,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     const int n = gather();
     cluster.sync();  // the lists are read
     if (n > kList) return false;
-    sort_descending(s.all, n);
+    sort_descending(s.all, n, s.list, s, list_bin(lo_bin, hi_bin));
     unsigned long long lw[kPer], l_all;
     running(n, lw, l_all);
     if (!(static_cast<double>(over) < reach) || static_cast<double>(over + l_all) < reach) return false;
@@ -773,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     const int n = gather();
     cluster.sync();  // the lists are read
     if (n <= kList) {
-      sort_descending(s.all, n);
+      sort_descending(s.all, n, s.list, s, list_bin(bin, bin));
       unsigned long long w[kPer] = {}, all;
       if (by_weight) running(n, w, all);
       settle(n, w, [&](int j, unsigned long long before) {
