@@ -79,7 +79,7 @@ class _Workspaces:
         self._retired: list[torch.Tensor] = []
         self.current_lane = 0
 
-    def get(self, device: torch.device, name: str, nbytes: int) -> torch.Tensor:
+    def get(self, device: torch.device, name, nbytes: int) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         key = (idx, name, self.current_lane)
         buf = self._bufs.get(key)
@@ -91,6 +91,10 @@ class _Workspaces:
             buf = torch.zeros(nb, dtype=torch.uint8, device=device)
             self._bufs[key] = buf
         return buf
+
+    def has(self, device: torch.device, name) -> bool:
+        idx = device.index if device.index is not None else torch.cuda.current_device()
+        return (idx, name, self.current_lane) in self._bufs
 
     @contextlib.contextmanager
     def lane(self, lane: int):
@@ -884,7 +888,10 @@ class PageStep:
 
 
 # These launches are short next to their host side, so its checks are kept to one call per
-# tensor and property (stride() and shape whole, get_device(), the raw stream).
+# tensor and property (stride() and shape whole, get_device(), the raw stream).  Their
+# workspaces hold counters that have to be zero between calls, so every stream has its own,
+# and recorded calls one per lane (graphs that may replay at the same time are recorded in
+# different lanes).
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
@@ -909,6 +916,19 @@ def _paged_bytes() -> tuple[int, int]:
     lib = _lib.load()
     return (lib.ddt_page_tables_workspace_bytes(_lib.DDT_MAX_PAGED_REQUESTS),
             lib.ddt_paged_attn_workspace_bytes(1 << 20, 1 << 20, 64, 1))
+
+
+def _stream_workspace(device: torch.device, name: str, stream: int, nbytes: int) -> torch.Tensor:
+    """The zeroed workspace of (device, lane, stream), or, while a graph is recorded, of (device,
+    lane)'s recorded calls.  That one is made beside the first call's own: memory allocated during
+    a recording would be zeroed by that graph's replays only."""
+    if not torch.cuda.is_current_stream_capturing():
+        if not WORKSPACES.has(device, (name, stream)):
+            WORKSPACES.get(device, (name, "recorded"), nbytes)
+        return WORKSPACES.get(device, (name, stream), nbytes)
+    if not WORKSPACES.has(device, (name, "recorded")):
+        raise _lib.DDTreeError(f"{name}: call it once on this device and lane before recording it")
+    return WORKSPACES.get(device, (name, "recorded"), nbytes)
 
 
 def _table_view(block_table: torch.Tensor, requests: int) -> tuple[int, int]:
@@ -951,13 +971,14 @@ def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     if status is None:
         status = attention_status(old_lens.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(old_lens.device, "page_tables", _paged_bytes()[0])
+    stream = _raw_stream(idx)
+    ws = _stream_workspace(old_lens.device, "page_tables", stream, _paged_bytes()[0])
     check(lib.ddt_page_tables(
         old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(), t_stride, cols,
         page_size, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
         out.kv_lens.data_ptr(), out.cu_new.data_ptr(), out.slot_map.data_ptr(),
         out.positions.data_ptr(), max_tokens, out.free_count.data_ptr(), ws.data_ptr(),
-        ws.numel(), status.data_ptr(), _raw_stream(idx)), "ddt_page_tables")
+        ws.numel(), status.data_ptr(), stream), "ddt_page_tables")
     STATS.launches += 1
     return out
 
@@ -1042,13 +1063,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if status is None:
         status = attention_status(q.device)
     lib = _lib.load()
-    ws = WORKSPACES.get(q.device, "paged_attn", _paged_bytes()[1])
+    stream = _raw_stream(idx)
+    ws = _stream_workspace(q.device, "paged_attn", stream, _paged_bytes()[1])
     check(lib.ddt_paged_attn(
         q.data_ptr(), q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
         ps, sp, sh, sr, block_table.data_ptr(), t_stride, cols, cu_new.data_ptr(),
         kv_lens.data_ptr(), R, T, max_new, hq, hkv, d, d ** -0.5 if scale is None else scale,
         out.data_ptr(), o_strides[0], o_strides[1], ws.data_ptr(), ws.numel(), status.data_ptr(),
-        _raw_stream(idx)), "ddt_paged_attn")
+        stream), "ddt_paged_attn")
     STATS.launches += 1
     return out
 

@@ -430,6 +430,32 @@ def test_paged_attention_far_pages(cuda_device):
     c.check(out)
 
 
+def test_paged_kernels_on_two_streams_at_once(cuda_device):
+    """Calls that overlap on two streams share no scratch: 30 rounds of cut units and page steps on
+    each, all equal to what either gives alone."""
+    cases = [_Case(cuda_device, [5000, 3000], [1, 1], 32, 8, 16, seed=1),
+             _Case(cuda_device, [4000, 900], [1, 300], 32, 8, 16, seed=2)]
+    alone = [c.run() for c in cases]
+    lens = [_i32(c.lens, cuda_device) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[], []]
+    steps = [[], []]
+    for _ in range(30):
+        for i, (c, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                outs[i].append(c.run())
+                steps[i].append(K.page_tables(torch.zeros_like(lens[i]), lens[i], c.table.clone(),
+                                              torch.arange(1000, dtype=torch.int32, device=cuda_device),
+                                              _i32([1000], cuda_device), 16, 9000))
+    torch.cuda.synchronize()
+    for i, c in enumerate(cases):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+        for st in steps[i]:
+            assert st.kv_lens.tolist() == c.lens and int(st.slot_map.max()) < 16000
+            assert int((st.slot_map >= 0).sum()) == sum(c.lens)
+
+
 def test_paged_attention_mixed_batch_recorded(cuda_device):
     """Both kernels and the merge in a recorded graph, on a side stream, replayed back to back."""
     lens, news, hq, hkv, page = ATTN["chunk_among_30"]
@@ -447,6 +473,24 @@ def test_paged_attention_mixed_batch_recorded(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, eager) for o in outs)
+
+
+def test_paged_attention_recorded_without_a_first_call_is_refused(cuda_device):
+    c = _Case(cuda_device, [70, 9], [3, 2], 8, 2, 16)
+    graph = torch.cuda.CUDAGraph()
+    with K.WORKSPACES.lane(971):
+        with pytest.raises(_lib.DDTreeError, match="before recording"):
+            with torch.cuda.graph(graph):
+                c.q.add_(0)
+                c.run()
+        c.run()  # and with one it records
+        out = torch.zeros_like(c.q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.run(out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    c.check(out)
 
 
 @pytest.mark.parametrize("news", [[1, 1, 1, 1], [16, 3, 16, 1], [100, 1, 300, 64]])

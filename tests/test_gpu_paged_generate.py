@@ -137,6 +137,43 @@ def test_paged_generate_samples_reproducibly_and_stops(cuda_device, runner):
     assert first <= 7
 
 
+def test_recorded_decode_step_serves_growing_requests(cuda_device, runner):
+    """Page tables, forward and sampling of a decode step recorded in one graph, replayed while
+    the requests grow across pages: the tokens of the eager loop."""
+    dev = cuda_device
+    prompts = [torch.arange(30), torch.arange(7), torch.arange(64)]
+    want = paged_generate(runner, prompts, 24, page_size=16)
+    cache = PagedKVCache(2, 24, 2, 128, 3, 8, 16, dev)
+    ids = torch.cat(prompts).to(dev)
+    step = cache.step(torch.tensor([30, 7, 64], dtype=torch.int32, device=dev), 101)
+    f32 = dict(dtype=torch.float32, device=dev)
+    u, temp = torch.zeros(3, **f32), torch.zeros(3, **f32)
+    with torch.inference_mode():
+        logits = runner.forward_paged(ids, cache, step, 64, torch.tensor([29, 36, 100], device=dev))
+        token = K.sample(logits, u, temp)[0].clone()
+        got = [token.tolist()]
+
+        def decode():
+            st = cache.step(cache.lens + 1, 3)
+            K.sample(runner.forward_paged(token, cache, st, 1), u, temp, out=token)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # warms up and decodes one token
+            decode()
+        torch.cuda.current_stream().wait_stream(side)
+        got.append(token.tolist())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            decode()
+        for _ in range(22):
+            graph.replay()
+            got.append(token.tolist())
+    cache.check()
+    assert cache.lens.tolist() == [53, 30, 87]
+    assert [list(t) for t in zip(*got)] == [w.tolist() for w in want]
+
+
 def test_paged_cache_reports_an_exhausted_pool(cuda_device):
     cache = PagedKVCache(1, 4, 1, 128, 2, 8, 16, cuda_device)
     st = cache.step(torch.tensor([40, 60], dtype=torch.int32, device=cuda_device), 100)
