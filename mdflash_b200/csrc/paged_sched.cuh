@@ -2,10 +2,11 @@
 // lengths (no plan is built on the host or kept between calls, so one recorded launch serves
 // every length).
 //
-// A unit is (KV head, request, up to kTokens consecutive new tokens of it); it attends to the
+// A unit is (KV head, request, up to so many consecutive new tokens of it); it attends to the
 // keys [0, past + its last token + 1) in tiles of kTile keys.  Its cost is its tiles plus kItem
-// (loading Q, filling the pipeline, the epilogue; 2 tiles' worth measured for the tree
-// attention).  The units of all heads, head by head, form one line of W cost positions that is
+// (loading Q, filling the pipeline, the masked tiles, the epilogue).  Fitted over the CTAs of four
+// chunks of up to 2048 tokens it is 2.7 tiles of 128 keys, but 3 gains 0.8% there and costs blocks
+// of 16 tokens, whose tiles go two at a time, 4%.  The units of all heads, head by head, form one line of W cost positions that is
 // cut into equal pieces, one per CTA; a CTA runs the tiles that lie in its piece.  A unit that
 // crosses a cut is finished in parts: the part that holds the unit's first tile goes to slot
 // 2 c + 1 of its CTA c, every later one to slot 2 c of its CTA; they are consecutive CTAs, and
