@@ -230,8 +230,9 @@ extern "C" int ddt_page_tables(const int32_t* old_lens, const int32_t* new_lens,
                                int32_t* cu_new, int64_t* slot_map, int64_t* positions,
                                int64_t max_tokens, int32_t* free_count_out, void* workspace,
                                size_t workspace_bytes, int32_t* status, void* stream) {
-  if (!old_lens || !new_lens || !block_table || !free_pages || !free_count || !kv_lens ||
-      !cu_new || !free_count_out || (max_tokens > 0 && (!slot_map || !positions)))
+  if (!old_lens || !new_lens || !block_table || (free_capacity > 0 && !free_pages) ||
+      !free_count || !kv_lens || !cu_new || !free_count_out ||
+      (max_tokens > 0 && (!slot_map || !positions)))
     return DDT_ERR_INVALID;
   if (n_requests <= 0 || max_pages <= 0 || table_stride < max_pages || max_tokens < 0 ||
       free_capacity < 0)

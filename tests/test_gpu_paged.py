@@ -131,6 +131,12 @@ def test_page_tables_take_pages_given_back_in_the_same_step(cuda_device):
     assert _run_tables(cuda_device, [64, 0, 48], [0, 112, 0], 16, 7, 0, 112)
 
 
+def test_page_tables_of_requests_without_pages(cuda_device):
+    # nothing held, nothing wanted, and a free stack of no entries at all
+    assert _run_tables(cuda_device, [0, 0, 0], [0, 0, 0], 16, 3, 0, 0)
+    assert not _run_tables(cuda_device, [0, 0, 0], [0, 1, 0], 16, 3, 0, 4)
+
+
 @pytest.mark.parametrize("old,new,spare,max_tokens", [
     ([10, 20], [60, 70], 5, 200),    # 6 pages wanted, 5 free
     ([10, 20], [12, 200], 50, 300),  # beyond max_pages
