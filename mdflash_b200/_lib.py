@@ -10,6 +10,7 @@ import os
 from . import build as _build
 
 _lib = None
+_binding = None
 
 DDT_OK = 0
 DDT_ERR_TIMEOUT = -6
@@ -134,6 +135,21 @@ def load(build_if_missing: bool = True):
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def binding():
+    """The compiled Python binding (_bind.so) of the entry points whose host side outweighs their
+    kernels; built and loaded like the library, which it calls."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _bind
+        except ImportError as e:
+            raise DDTreeError(f"ddtree_b200 Python binding cannot be loaded: {e}; run "
+                              "`python -m mdflash_b200.build`") from e
+        _binding = _bind
+    return _binding
 
 
 def check(rc: int, what: str) -> None:

@@ -92,9 +92,8 @@ class _Workspaces:
             self._bufs[key] = buf
         return buf
 
-    def has(self, device: torch.device, name) -> bool:
-        idx = device.index if device.index is not None else torch.cuda.current_device()
-        return (idx, name, self.current_lane) in self._bufs
+    def find(self, idx: int, name) -> torch.Tensor | None:
+        return self._bufs.get((idx, name, self.current_lane))
 
     @contextlib.contextmanager
     def lane(self, lane: int):
@@ -887,26 +886,12 @@ class PageStep:
         return PageStep(lens, cu_new, slots, positions, count)
 
 
-# These launches are short next to their host side, so its checks are kept to one call per
-# tensor and property (stride() and shape whole, get_device(), the raw stream).  Their
-# workspaces hold counters that have to be zero between calls, so every stream has its own,
-# and recorded calls one per lane (graphs that may replay at the same time are recorded in
-# different lanes).
+# These launches are shorter than their host side, so their checks, outputs and launch are one call
+# of the compiled binding (csrc/bind.cpp).  Their workspaces hold counters that have to be zero
+# between calls, so every stream has its own, and recorded calls one per lane (graphs that may
+# replay at the same time are recorded in different lanes).
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
-
-
-def _device_of(*ts: torch.Tensor) -> int:
-    idx = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != idx or idx < 0:
-            _require_cuda(*ts)
-    return idx
-
-
-def _need(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None:
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
 
 
 @functools.cache
@@ -918,26 +903,24 @@ def _paged_bytes() -> tuple[int, int]:
             lib.ddt_paged_attn_workspace_bytes(1 << 20, 1 << 20, 64, 1))
 
 
-def _stream_workspace(device: torch.device, name: str, stream: int, nbytes: int) -> torch.Tensor:
-    """The zeroed workspace of (device, lane, stream), or, while a graph is recorded, of (device,
-    lane)'s recorded calls.  That one is made beside the first call's own: memory allocated during
-    a recording would be zeroed by that graph's replays only."""
-    if not torch.cuda.is_current_stream_capturing():
-        if not WORKSPACES.has(device, (name, stream)):
-            WORKSPACES.get(device, (name, "recorded"), nbytes)
-        return WORKSPACES.get(device, (name, stream), nbytes)
-    if not WORKSPACES.has(device, (name, "recorded")):
-        raise _lib.DDTreeError(f"{name}: call it once on this device and lane before recording it")
-    return WORKSPACES.get(device, (name, "recorded"), nbytes)
-
-
-def _table_view(block_table: torch.Tensor, requests: int) -> tuple[int, int]:
-    """(row stride, columns) of a block table i32 [requests, max_pages]."""
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
-            block_table.shape[0] != requests or block_table.stride(1) != 1:
-        raise ValueError("block_table must be i32 [requests, max_pages] with unit stride")
-    cols = block_table.shape[1]
-    return (block_table.stride(0) if requests > 1 else cols), cols
+def _stream_workspace(t: torch.Tensor, name: str, nbytes: int) -> torch.Tensor:
+    """The zeroed workspace of (t's device, lane, current stream), or, while a graph is recorded, of
+    (device, lane)'s recorded calls.  That one is made beside the first call's own: memory allocated
+    during a recording would be zeroed by that graph's replays only."""
+    idx = t.get_device()
+    if idx < 0:
+        _require_cuda(t)
+    if torch.cuda.is_current_stream_capturing():
+        ws = WORKSPACES.find(idx, (name, "recorded"))
+        if ws is None:
+            raise _lib.DDTreeError(f"{name}: call it once on this device and lane before recording it")
+        return ws
+    stream = _raw_stream(idx)
+    ws = WORKSPACES.find(idx, (name, stream))
+    if ws is None:
+        WORKSPACES.get(t.device, (name, "recorded"), nbytes)
+        ws = WORKSPACES.get(t.device, (name, stream), nbytes)
+    return ws
 
 
 def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -951,49 +934,14 @@ def page_tables(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     out.free_count (which may be free_count; out.kv_lens may be old_lens or new_lens).
     max_tokens bounds the step's new tokens.  A step that does not fit changes nothing and
     reports itself in the status word (check_status)."""
-    idx = _device_of(old_lens, new_lens, block_table, free_pages, free_count)
-    R = old_lens.numel()
-    _need(old_lens, torch.int32, (R,), "old_lens")
-    _need(new_lens, torch.int32, (R,), "new_lens")
-    _need(free_count, torch.int32, (1,), "free_count")
-    t_stride, cols = _table_view(block_table, R)
-    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
-        raise ValueError("free_pages must be a contiguous i32 vector")
-    if out is None:
-        out = PageStep.allocate(old_lens.device, R, max_tokens)
-    else:
-        _device_of(old_lens, out.kv_lens, out.cu_new, out.slot_map, out.positions, out.free_count)
-        _need(out.kv_lens, torch.int32, (R,), "out.kv_lens")
-        _need(out.cu_new, torch.int32, (R + 1,), "out.cu_new")
-        _need(out.slot_map, torch.int64, (max_tokens,), "out.slot_map")
-        _need(out.positions, torch.int64, (max_tokens,), "out.positions")
-        _need(out.free_count, torch.int32, (1,), "out.free_count")
-    if status is None:
-        status = attention_status(old_lens.device)
-    lib = _lib.load()
-    stream = _raw_stream(idx)
-    ws = _stream_workspace(old_lens.device, "page_tables", stream, _paged_bytes()[0])
-    check(lib.ddt_page_tables(
-        old_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(), t_stride, cols,
-        page_size, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(),
-        out.kv_lens.data_ptr(), out.cu_new.data_ptr(), out.slot_map.data_ptr(),
-        out.positions.data_ptr(), max_tokens, out.free_count.data_ptr(), ws.data_ptr(),
-        ws.numel(), status.data_ptr(), stream), "ddt_page_tables")
+    ws = _stream_workspace(old_lens, "page_tables", _paged_bytes()[0])
+    step = _lib.binding().page_tables(
+        old_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens,
+        None if out is None else (out.kv_lens, out.cu_new, out.slot_map, out.positions,
+                                  out.free_count),
+        attention_status(old_lens.device) if status is None else status, ws)
     STATS.launches += 1
-    return out
-
-
-def _pages_view(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, ...]:
-    """(n_pages, kv_heads, page_size, head_dim, page stride, head stride, row stride) of a page
-    pool: logical [pages, kv_heads, page_size, head_dim] bf16 with any strides but the last."""
-    strides = k_pages.stride()
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or strides != v_pages.stride() or \
-            strides[3] != 1:
-        raise ValueError("k_pages / v_pages must be [pages, kv_heads, page_size, head_dim] with "
-                         "the same strides and contiguous rows")
-    if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
-        raise TypeError("paged K/V are bf16")
-    return *k_pages.shape, *strides[:3]
+    return PageStep(*step) if out is None else out
 
 
 def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
@@ -1004,33 +952,10 @@ def paged_qk_norm_rope(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torc
     qkv [T, (q_heads + 2 kv_heads) * 128] (bf16), K / V rows into slot slot_map[i] (i64 [>= T];
     -1 writes none) of the page pool [pages, kv_heads, page_size, 128].  rope_table i32 [T, 64]
     (ddt_rope_table).  Returns q [T, q_heads, 128]."""
-    idx = _device_of(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages, v_pages)
-    n_pages, hkv, ps, d, sp, sh, sr = _pages_view(k_pages, v_pages)
-    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or qkv.shape[1] % d:
-        raise ValueError("qkv must be bf16 [tokens, heads * head_dim] with unit stride")
-    T, width = qkv.shape
-    hq = width // d - 2 * hkv
-    if hq <= 0:
-        raise ValueError("qkv holds no query heads beside the pool's KV heads")
-    if q_norm_w.dtype != torch.bfloat16 or k_norm_w.dtype != torch.bfloat16 or \
-            q_norm_w.shape != (d,) or k_norm_w.shape != (d,):
-        raise ValueError("norm weights must be bf16 [head_dim]")
-    _need(rope_table, torch.int32, (T, d // 2), "rope_table")
-    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or slot_map.shape[0] < T or \
-            not slot_map.is_contiguous():
-        raise ValueError("slot_map must be contiguous i64 with a slot per token")
-    if out is None:
-        out = qkv.new_empty((T, hq, d))
-    else:
-        _need(out, torch.bfloat16, (T, hq, d), "out")
-        _device_of(qkv, out)
-    check(_lib.load().ddt_paged_qk_norm_rope(
-        qkv.data_ptr(), max(qkv.stride(0), width), T, hq, hkv, d, q_norm_w.data_ptr(),
-        k_norm_w.data_ptr(), eps, rope_table.data_ptr(), slot_map.data_ptr(), out.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, sp, sh, sr, _raw_stream(idx)),
-        "ddt_paged_qk_norm_rope")
+    q = _lib.binding().paged_qk_norm_rope(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages,
+                                          v_pages, eps, out)
     STATS.launches += 1
-    return out
+    return q
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -1042,37 +967,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (the new rows' K / V are already in the pool); max_new is the host's bound on the new
     tokens of one request.  Returns [T, q_heads, 128]; rows that no request owns are not
     written."""
-    idx = _device_of(q, k_pages, v_pages, block_table, cu_new, kv_lens)
-    n_pages, hkv, ps, d, sp, sh, sr = _pages_view(k_pages, v_pages)
-    q_strides = q.stride()
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q_strides[2] != 1:
-        raise ValueError("q must be bf16 [tokens, q_heads, head_dim] with contiguous rows")
-    T, hq, qd = q.shape
-    if qd != d:
-        raise ValueError("q and the pages differ in head_dim")
-    R = kv_lens.numel()
-    _need(kv_lens, torch.int32, (R,), "kv_lens")
-    _need(cu_new, torch.int32, (R + 1,), "cu_new")
-    t_stride, cols = _table_view(block_table, R)
-    if out is None:
-        out = q.new_empty((T, hq, d))
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
-            out.get_device() != idx:
-        raise ValueError("out must be like q")
-    o_strides = out.stride()
-    if status is None:
-        status = attention_status(q.device)
-    lib = _lib.load()
-    stream = _raw_stream(idx)
-    ws = _stream_workspace(q.device, "paged_attn", stream, _paged_bytes()[1])
-    check(lib.ddt_paged_attn(
-        q.data_ptr(), q_strides[0], q_strides[1], k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
-        ps, sp, sh, sr, block_table.data_ptr(), t_stride, cols, cu_new.data_ptr(),
-        kv_lens.data_ptr(), R, T, max_new, hq, hkv, d, d ** -0.5 if scale is None else scale,
-        out.data_ptr(), o_strides[0], o_strides[1], ws.data_ptr(), ws.numel(), status.data_ptr(),
-        stream), "ddt_paged_attn")
+    ws = _stream_workspace(q, "paged_attn", _paged_bytes()[1])
+    o = _lib.binding().paged_attention(
+        q, k_pages, v_pages, block_table, cu_new, kv_lens, max_new, scale, out,
+        attention_status(q.device) if status is None else status, ws)
     STATS.launches += 1
-    return out
+    return o
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
@@ -1083,32 +983,6 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
     uniforms u f32 [rows], with per-row temperature f32, top_k i32, top_p f32 and min_p f32
     (None: off).  Returns (tokens i64 [rows], logprobs f32 [rows]); -1 and -inf for a row
     without a token to draw."""
-    idx = _device_of(logits, u, temperature)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("logits must be [rows, vocab] with unit stride")
-    rows, vocab = logits.shape
-    _need(u, torch.float32, (rows,), "u")
-    _need(temperature, torch.float32, (rows,), "temperature")
-    rules = []
-    for t, dt, name in ((top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
-                        (min_p, torch.float32, "min_p")):
-        if t is not None:
-            _device_of(logits, t)
-            _need(t, dt, (rows,), name)
-        rules.append(None if t is None else t.data_ptr())
-    if out is None:
-        out = u.new_empty(rows, dtype=torch.int64)
-    else:
-        _device_of(logits, out)
-        _need(out, torch.int64, (rows,), "out")
-    if logprobs is None:
-        logprobs = u.new_empty(rows)
-    else:
-        _device_of(logits, logprobs)
-        _need(logprobs, torch.float32, (rows,), "logprobs")
-    check(_lib.load().ddt_sample(
-        logits.data_ptr(), _dtype_code(logits), rows, vocab, max(logits.stride(0), vocab),
-        u.data_ptr(), temperature.data_ptr(), *rules, out.data_ptr(), logprobs.data_ptr(),
-        _raw_stream(idx)), "ddt_sample")
+    drawn = _lib.binding().sample(logits, u, temperature, top_k, top_p, min_p, out, logprobs)
     STATS.launches += 1
-    return out, logprobs
+    return drawn

@@ -554,3 +554,33 @@ def test_paged_refusals(cuda_device):
         K.paged_attention(c.q, odd, odd, c.table, c.cu_new, c.kv_lens, 3)
     assert K.paged_attention(c.q[:0], c.k_pages, c.v_pages, c.table, c.cu_new, c.kv_lens,
                              0).shape == (0, 8, D)
+
+
+def test_paged_calls_refuse_what_the_kernels_would_misread(cuda_device):
+    c = _Case(cuda_device, [70, 9], [3, 2], 8, 2, 16)
+    for status in (torch.zeros(1, dtype=torch.int32),
+                   torch.zeros(1, dtype=torch.int64, device=cuda_device),
+                   torch.zeros(0, dtype=torch.int32, device=cuda_device)):
+        with pytest.raises(ValueError):
+            c.run(status=status)
+        with pytest.raises(ValueError):
+            K.page_tables(_i32([0], cuda_device), _i32([4], cuda_device), _i32([[0]], cuda_device),
+                          _i32([0], cuda_device), _i32([1], cuda_device), 16, 4, status=status)
+    with pytest.raises(ValueError):
+        K.page_tables(_i32([0], cuda_device), _i32([4], cuda_device), _i32([[0]], cuda_device),
+                      _i32([0], cuda_device), _i32([1], cuda_device), 16, -1)
+    step = K.PageStep.allocate(cuda_device, 1, 3)
+    with pytest.raises(ValueError, match="out.slot_map"):  # made for 3 tokens
+        K.page_tables(_i32([0], cuda_device), _i32([4], cuda_device), _i32([[0]], cuda_device),
+                      _i32([0], cuda_device), _i32([1], cuda_device), 16, 4, out=step)
+    w = torch.ones(2 * D, dtype=torch.bfloat16, device=cuda_device)
+    rope = torch.zeros((4, D // 2), dtype=torch.int32, device=cuda_device)
+    qkv = torch.zeros((4, 12 * D), dtype=torch.bfloat16, device=cuda_device)
+    slots = torch.full((4,), -1, dtype=torch.int64, device=cuda_device)
+    K.paged_qk_norm_rope(qkv, w[:D], w[:D], rope, slots, c.k_pages, c.v_pages)
+    with pytest.raises(ValueError, match="norm weights"):  # every other element
+        K.paged_qk_norm_rope(qkv, w[::2], w[:D], rope, slots, c.k_pages, c.v_pages)
+    with pytest.raises(ValueError, match="slot"):
+        K.paged_qk_norm_rope(qkv, w[:D], w[:D], rope, slots[:3], c.k_pages, c.v_pages)
+    with pytest.raises(ValueError, match="out"):
+        K.paged_qk_norm_rope(qkv, w[:D], w[:D], rope, slots, c.k_pages, c.v_pages, out=qkv)

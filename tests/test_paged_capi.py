@@ -70,3 +70,19 @@ SAMPLE_OK = dict(x=P, dtype=1, rows=2, vocab=100, rs=100, u=P, temp=P, k=P, p=P,
     (dict(vocab=1 << 22, rs=1 << 22), -2), (dict(x=ctypes.c_void_p(257)), -4), (dict(rows=0, x=None), 0)])
 def test_sample_refusals(change, code):
     assert _call("ddt_sample", SAMPLE, SAMPLE_OK, **change) == code
+
+
+def test_binding_refuses_host_tensors_and_wrong_kinds():
+    torch = pytest.importorskip("torch")
+    from mdflash_b200 import kernels as K
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        K.page_tables(i, i, i.view(1, 1), i, i, 16, 4)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        K.paged_qk_norm_rope(i, i, i, i, i, i, i)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        K.paged_attention(i, i, i, i, i, i, 1)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        K.sample(i, i, i)
+    with pytest.raises(TypeError):
+        K.sample(None, i, i)
