@@ -195,12 +195,14 @@ __global__ void __launch_bounds__(kThreads, 1) page_tables_kernel(const TableArg
   // the last CTA writes what may alias an input: every CTA has read its inputs by then
   __shared__ bool s_last;
   __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    s_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  if (gridDim.x > 1) {
+    if (tid == 0) {
+      __threadfence();
+      s_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
   }
-  __syncthreads();
-  if (!s_last) return;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const int r = tid * kPer + k;
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) page_tables_kernel(const TableArg
   if (tid == 0) {
     *a.free_count_out = static_cast<int32_t>(ok ? count + n_back - n_more : count);
     if (!ok && a.status) atomicOr(a.status, DDT_STATUS_PAGES);
-    *a.ticket = 0u;
+    if (gridDim.x > 1) *a.ticket = 0u;
   }
 }
 
