@@ -19,6 +19,38 @@ inline int launch_status() {
   return e == cudaSuccess ? DDT_OK : DDT_ERR_CUDA;
 }
 
+// Launch that may begin while the kernel before it in the stream ends.  The kernel calls
+// after_stream() in every thread before it touches memory that others use, and let_next_begin()
+// where the next such launch may take the room that this one leaves.  (Recorded, 8 requests of 1000
+// keys: write and attention of one token each 16.0 to 14.7 us; one request's attention 10.5 to
+// 9.7 us.)
+template <typename... P, typename... A>
+inline int launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                        unsigned cluster, A... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess) return DDT_OK;
+  cudaGetLastError();
+  return DDT_ERR_CUDA;
+}
+__device__ __forceinline__ void after_stream() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ---- order-preserving keys ------------------------------------------------

@@ -136,6 +136,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     bars.abort = 0;
     tc::fence_mbar_init();
   }
+  // before the allocation: a kernel that is still running may have yet to take its TMEM
+  if (!p.beside) after_stream();
   if (warp == 1) {
     tc::tmem_alloc(&bars.tmem_base, kTmemCols);
     tc::tmem_relinquish();
@@ -146,7 +148,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   tc::tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
   // the merge kernel may be scheduled from here on (it waits for this grid's end)
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_begin();
   volatile int* abort_flag = &bars.abort;
   const Item& it = places[warp].it;  // the warp's current item
   auto next = [&] { return walk_next<kBlockN>(p, 2 * tile_tok, s_first, piece, places[warp]); };
@@ -681,7 +683,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
   // a short kernel launched before this one is over before this one is: what follows in the
   // stream waits for this one only
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_stream();
 }
 
 // ---- merge of the parts ----------------------------------------------------------------
@@ -694,7 +696,7 @@ constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const Params p) {
   const int c0 = blockIdx.x;
   // launched while the attention kernel still runs: its writes are there after this wait
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_stream();
   const int4 part = p.parts[c0];
   if (part.w < 0) return;
   const int w = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -861,30 +863,13 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kSms);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  // beside the short kernel's last CTAs: the two share no output
-  cfg.numAttrs = both ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, paged_attn_kernel, tm_q, tm_k, tm_v, p) != cudaSuccess) {
-    cudaGetLastError();
-    return DDT_ERR_CUDA;
-  }
-  // programmatic launch: the merge's CTAs take the SMs as the attention's leave them and wait
-  // there for its end, instead of being launched after it
-  cfg.gridDim = dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps);
-  cfg.blockDim = dim3(kMergeWarps * 32);
-  cfg.dynamicSmemBytes = 0;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, paged_merge_kernel, p) != cudaSuccess) {
-    cudaGetLastError();
-    return DDT_ERR_CUDA;
-  }
-  return DDT_OK;
+  // beside the few-rows kernel's last CTAs: the two share no output
+  p.beside = both;
+  rc = launch_early(paged_attn_kernel, dim3(kSms), dim3(kThreads), smem, st, 0, tm_q, tm_k, tm_v, p);
+  if (rc) return rc;
+  // the merge's CTAs take the SMs as the attention's leave them and wait there for its end,
+  // instead of being launched after it
+  return launch_early(paged_merge_kernel,
+                      dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
+                      dim3(kMergeWarps * 32), 0, st, 0, p);
 }

@@ -19,7 +19,7 @@
 // length may hold anything; their fragments are replaced by zeros in registers.
 // Measured, one token for each of 64 requests of 1k to 32k keys, 32 query heads over 8 (2.38 GB
 // of K and V): 362 us, 6.57 TB/s, the measured copy rate, with 1.003 times the bytes read from
-// HBM.  One request of 1000 keys takes 10.5 us, two thirds of it dependent reads (lengths, page
+// HBM.  One request of 1000 keys takes 9.7 us, two thirds of it dependent reads (lengths, page
 // ids, K, the parts).
 // Units are cut over the CTAs as in paged_sched.cuh; the CTA that brings a cut unit's last part
 // merges all of them, in the order of the CTAs, so the result does not depend on which it is.
@@ -190,11 +190,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     bars.abort = 0;
     tc::fence_mbar_init();
   }
+  after_stream();
   walk_begin<kKeys>(p, unit_tok, static_cast<long long>(kMaxParts / kM) * p.kv_heads * p.n_requests,
                     s_first, s_warp, piece, places, kConsumers + 1);
   __syncthreads();
-  // the other kernel of a mixed batch may take the SMs that this one leaves
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // the other kernel of a mixed batch may take the SMs that this one leaves; it reads what was
+  // written before this one, which is over by now
+  let_next_begin();
   volatile int* abort_flag = &bars.abort;
   const Item& it = places[warp].it;
   auto next = [&] { return walk_next<kKeys>(p, unit_tok, s_first, piece, places[warp]); };
@@ -505,8 +507,8 @@ int launch_m(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap
   if (cudaFuncSetAttribute(paged_decode_kernel<kM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  paged_decode_kernel<kM><<<kShortCtas, kShortThreads, smem, st>>>(tm_q, tm_k, tm_v, p, bufs);
-  return launch_status();
+  return launch_early(paged_decode_kernel<kM>, dim3(kShortCtas), dim3(kShortThreads), smem, st, 0, tm_q,
+                      tm_k, tm_v, p, bufs);
 }
 
 }  // namespace

@@ -37,6 +37,7 @@ struct Params {
   const int32_t* kv_lens;
   int n_requests, n_tokens, max_new, group, kv_heads;
   int from_new, to_new;  // the launch takes the requests with so many new tokens
+  int beside;            // launched beside the few-rows kernel, which waited for what is read here
   float scale_log2;
   __nv_bfloat16* out;
   long long o_token_stride, o_head_stride;

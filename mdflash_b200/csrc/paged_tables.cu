@@ -109,6 +109,8 @@ __global__ void __launch_bounds__(kThreads, 1) page_tables_kernel(const TableArg
       s_tok[DDT_MAX_PAGED_REQUESTS + 1];
   const int tid = threadIdx.x, n = a.n_requests;
   const long long page = 1ll << a.page_shift;
+  after_stream();
+  let_next_begin();
   int32_t old_len[kPer], new_len[kPer];
   long long v[kScans][kPer], total[kScans];
   auto &back = v[0], &more = v[1], &tok = v[2];
@@ -269,7 +271,6 @@ extern "C" int ddt_page_tables(const int32_t* old_lens, const int32_t* new_lens,
   const int64_t by_requests = (n_requests + 127) / 128;
   int64_t blocks = by_tokens > by_requests ? by_tokens : by_requests;
   if (blocks > 148) blocks = 148;
-  paged::page_tables_kernel<<<static_cast<unsigned>(blocks), paged::kThreads, 0,
-                              static_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status();
+  return launch_early(paged::page_tables_kernel, dim3(static_cast<unsigned>(blocks)),
+                      dim3(paged::kThreads), 0, static_cast<cudaStream_t>(stream), 0, a);
 }

@@ -228,6 +228,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
   const char* x = static_cast<const char*>(a.logits) + row * a.row_stride * (kBF16 ? 2 : 4);
   auto peer = [&](int r) { return cluster.map_shared_rank(&s, r); };
 
+  after_stream();
+  let_next_begin();
+
   // ---- the row's rules --------------------------------------------------------------------
   const float temp_in = a.temperature[row];
   const bool greedy = !(temp_in >= 1e-5f);
@@ -1058,20 +1061,7 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            sizeof(sample::Shared)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
-  cfg.blockDim = dim3(sample::kThreads);
-  cfg.dynamicSmemBytes = sizeof(sample::Shared);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
-    cudaGetLastError();
-    return DDT_ERR_CUDA;
-  }
-  return DDT_OK;
+  return launch_early(kernel, dim3(static_cast<unsigned>(rows * ranks)), dim3(sample::kThreads),
+                      sizeof(sample::Shared), static_cast<cudaStream_t>(stream),
+                      static_cast<unsigned>(ranks), a);
 }

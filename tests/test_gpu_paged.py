@@ -584,3 +584,63 @@ def test_paged_calls_refuse_what_the_kernels_would_misread(cuda_device):
         K.paged_qk_norm_rope(qkv, w[:D], w[:D], rope, slots[:3], c.k_pages, c.v_pages)
     with pytest.raises(ValueError, match="out"):
         K.paged_qk_norm_rope(qkv, w[:D], w[:D], rope, slots, c.k_pages, c.v_pages, out=qkv)
+
+
+def test_paged_calls_recorded_after_other_work(cuda_device):
+    """Every call recorded straight after a fill, a copy, a join of two streams and another of the
+    calls: launches that may begin before the work in front of them ends still read its results."""
+    c = _Case(cuda_device, [900, 70, 41], [1, 1, 1], 16, 4, 16, seed=3)
+    d = _Case(cuda_device, [900, 400, 41], [90, 200, 1], 16, 4, 16, seed=4)
+    logits = torch.randn((4, 5000), device=cuda_device)
+    u = torch.rand(4, device=cuda_device)
+    one = torch.ones(4, device=cuda_device)
+    token, logprob = K.sample(logits, u, one)
+    inputs = [(c.q, c.q.clone()), (d.q, d.q.clone()), (c.kv_lens, c.kv_lens.clone()),
+              (d.k_pages, d.k_pages.clone()), (logits, logits.clone())]
+    outs = [torch.zeros_like(c.q) for _ in range(2)] + [torch.zeros_like(d.q) for _ in range(2)]
+    side = torch.cuda.Stream()
+
+    def blank():
+        for t, _ in inputs:
+            t.zero_()
+
+    def restore():
+        for t, kept in inputs:
+            t.copy_(kept)
+
+    def joined():
+        blank()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            restore()
+        torch.cuda.current_stream().wait_stream(side)
+
+    c.run(out=outs[0])
+    d.run(out=outs[0].new_zeros(d.q.shape))
+    graph = torch.cuda.CUDAGraph()
+    drawn = []
+    with torch.cuda.graph(graph):
+        blank()
+        restore()
+        c.run(out=outs[0])
+        blank()
+        restore()
+        d.run(out=outs[2])
+        joined()
+        c.run(out=outs[1])
+        joined()
+        d.run(out=outs[3])
+        drawn.append(K.sample(logits, u, one))
+        joined()
+        drawn.append(K.sample(logits, u, one))
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    for o in outs[:2]:
+        c.check(o)
+    for o in outs[2:]:
+        d.check(o)
+    for t, lp in drawn:
+        assert torch.equal(t, token) and torch.equal(lp, logprob)
