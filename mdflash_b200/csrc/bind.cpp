@@ -51,6 +51,16 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType dtype, int idx) {
   return at::empty(shape, at::TensorOptions().dtype(dtype).device(at::Device(at::kCUDA, idx)));
 }
 
+// n elements of `dtype` from element `first` (of that type) on of the storage of `of`: one
+// allocation for several outputs, without a dispatched view for each (three times as long).
+Tensor part(const Tensor& of, int64_t first, int64_t n, at::ScalarType dtype) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(),
+                                                      c10::scalarTypeToTypeMeta(dtype));
+  t.unsafeGetTensorImpl()->set_storage_offset(first);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 template <typename T = void>
 T* ptr(const Tensor& t) {
   return static_cast<T*>(t.data_ptr());
@@ -116,14 +126,11 @@ Step page_tables(const Tensor& old_lens, const Tensor& new_lens, const Tensor& b
     need(positions, at::kLong, {max_tokens}, "out.positions");
     need(count, at::kInt, {1}, "out.free_count");
   } else {
-    // parts of two allocations (integers: nothing for autograd to track)
-    at::AutoDispatchBelowADInplaceOrView no_autograd;
-    const Tensor lens = fresh({2 * R + 2}, at::kInt, idx);
-    const Tensor tokens = fresh({2 * max_tokens}, at::kLong, idx);
-    o = Step(lens.as_strided({R}, {1}, 0), lens.as_strided({R + 1}, {1}, R),
-             tokens.as_strided({max_tokens}, {1}, 0),
-             tokens.as_strided({max_tokens}, {1}, max_tokens),
-             lens.as_strided({1}, {1}, 2 * R + 1));
+    const Tensor all = fresh({2 * max_tokens + R + 1}, at::kLong, idx);
+    const int64_t lens = 4 * max_tokens;  // the 32-bit parts start here
+    o = Step(part(all, lens, R, at::kInt), part(all, lens + R, R + 1, at::kInt),
+             part(all, 0, max_tokens, at::kLong), part(all, max_tokens, max_tokens, at::kLong),
+             part(all, lens + 2 * R + 1, 1, at::kInt));
   }
   const auto& [kv_lens, cu_new, slots, positions, count] = o;
   check(ddt_page_tables(ptr<int32_t>(old_lens), ptr<int32_t>(new_lens), R, ptr<int32_t>(block_table),

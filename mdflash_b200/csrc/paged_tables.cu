@@ -14,8 +14,8 @@
 // Every CTA scans the lengths of all requests itself (at most 2048 of them, two per thread)
 // and then covers its share of the pages and tokens; the grid's last CTA (a ticket, no waiting)
 // writes the outputs that may alias inputs.  Bound by latency: a step of 64 decoding requests
-// is one CTA and a few dependent reads, 6.0 us in a recorded graph; 1000 requests with 49k new
-// tokens (1 MB in and out) take 9.4 us (109 on one CTA).
+// is one CTA and a few dependent reads, 5.3 us in a recorded graph; 1000 requests with 49k new
+// tokens (1 MB in and out) take 9.2 us (109 on one CTA).
 #include "common.cuh"
 
 namespace ddt {

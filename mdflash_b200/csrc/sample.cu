@@ -23,7 +23,7 @@
 //
 // Measured over 151936 logits: one fp32 row with top-k 50 and top-p 0.95 18 us, with top-p alone
 // 30 us, untruncated 12 us (all latency: passes of 3 to 8 us, barriers and remote reads between
-// them); 64 bf16 rows of mixed rules 55 us (the slowest row); 257 fp32 rows untruncated 83 us,
+// them); 64 bf16 rows of mixed rules 55 us (the slowest row); 257 fp32 rows untruncated 82 us,
 // 1.9 TB/s: the exponential, its quotient and the split into whole numbers are 25 instructions
 // per logit, and rows in step read HBM and compute in turn.
 #include <cooperative_groups.h>
@@ -1051,7 +1051,7 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   sample::Args a{logits, static_cast<int>(vocab), row_stride, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs, aligned(logits, 16) && (row_stride * size) % 16 == 0};
   // as many CTAs per row as keep the rows in one wave (two CTAs per SM), or the rows in flight
-  // in L2 (they are read again; 257 rows of 608 KB: 83 us with 2 CTAs each, 95 with 4), and no
+  // in L2 (they are read again; 257 rows of 608 KB: 82 us with 2 CTAs each, 95 with 4), and no
   // more than leave each thread one load
   int ranks = 1;
   while (ranks < sample::kMaxCluster && vocab > ranks * sample::kThreads * (16 / size) &&

@@ -644,3 +644,29 @@ def test_paged_calls_recorded_after_other_work(cuda_device):
         d.check(o)
     for t, lp in drawn:
         assert torch.equal(t, token) and torch.equal(lp, logprob)
+
+
+def test_page_step_outputs_are_ordinary_tensors(cuda_device):
+    """They share one allocation: each keeps it alive, and views, copies and torch operations see
+    only its own elements."""
+    step = K.page_tables(_i32([0, 15], cuda_device), _i32([3, 17], cuda_device),
+                         _i32([[-1, -1], [6, -1]], cuda_device), _i32([9, 8, 7], cuda_device),
+                         _i32([3], cuda_device), 16, 7)
+    kv, cu, slots, pos, count = (step.kv_lens, step.cu_new, step.slot_map, step.positions,
+                                 step.free_count)
+    del step
+    assert [t.dtype for t in (kv, cu, slots, pos, count)] == [torch.int32] * 2 + [torch.int64] * 2 + \
+        [torch.int32]
+    assert [tuple(t.shape) for t in (kv, cu, slots, pos, count)] == [(2,), (3,), (7,), (7,), (1,)]
+    assert all(t.is_contiguous() and t.is_cuda and not t.requires_grad
+               for t in (kv, cu, slots, pos, count))
+    want = [112, 113, 114, 111, 128, -1, -1]
+    assert slots.tolist() == want and slots[2:].clone().tolist() == want[2:]
+    assert pos.view(7, 1).squeeze(1).tolist() == [0, 1, 2, 15, 16, 0, 0]
+    pos.fill_(5)
+    kv.add_(cu[1:])
+    del slots
+    torch.empty(1 << 20, device=cuda_device).fill_(1.0)
+    assert pos.tolist() == [5] * 7
+    assert kv.tolist() == [6, 22] and cu.tolist() == [0, 3, 5] and count.tolist() == [1]
+    assert torch.cat([kv, cu]).tolist() == [6, 22, 0, 3, 5]
