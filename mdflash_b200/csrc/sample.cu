@@ -1050,12 +1050,14 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   if (!aligned(logits, size)) return DDT_ERR_ALIGN;
   sample::Args a{logits, static_cast<int>(vocab), row_stride, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs, aligned(logits, 16) && (row_stride * size) % 16 == 0};
-  // as many CTAs per row as keep the rows in one wave (two CTAs per SM), or the rows in flight
-  // in L2 (they are read again; 257 rows of 608 KB: 82 us with 2 CTAs each, 95 with 4), and no
-  // more than leave each thread one load
+  // as many CTAs per row as keep the rows in one wave (two CTAs per SM; of the clusters of eight,
+  // whose SMs are neighbours, no more than 13: 24 fp32 rows with top-k and top-p take 18.9 us with
+  // 4 CTAs each, 24.9 with 8, and 32 rows 20.3 and 32.8; 13 rows with top-p alone 38.2 with 4, 31.0
+  // with 8), or the rows in flight in L2 (they are read again; 257 rows of 608 KB: 82 us with 2
+  // CTAs each, 95 with 4), and no more than leave each thread one load
   int ranks = 1;
   while (ranks < sample::kMaxCluster && vocab > ranks * sample::kThreads * (16 / size) &&
-         (rows * ranks * 2 <= 2 * 148 || 2 * 148 / ranks * vocab * size > (int64_t(100) << 20)))
+         (rows * ranks * 2 <= (ranks < 4 ? 2 * 148 : 104) || 2 * 148 / ranks * vocab * size > (int64_t(100) << 20)))
     ranks *= 2;
   auto kernel = dtype == DDT_BF16 ? sample::sample_kernel<true> : sample::sample_kernel<false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
