@@ -1057,7 +1057,8 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
   // CTAs each, 95 with 4), and no more than leave each thread one load
   int ranks = 1;
   while (ranks < sample::kMaxCluster && vocab > ranks * sample::kThreads * (16 / size) &&
-         (rows * ranks * 2 <= (ranks < 4 ? 2 * 148 : 104) || 2 * 148 / ranks * vocab * size > (int64_t(100) << 20)))
+         (rows * ranks * 2 <= (ranks < 4 ? 2 * 148 : 104) ||
+          2 * 148 / ranks * vocab * size > (int64_t(100) << 20)))
     ranks *= 2;
   auto kernel = dtype == DDT_BF16 ? sample::sample_kernel<true> : sample::sample_kernel<false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
