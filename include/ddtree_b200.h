@@ -523,9 +523,10 @@ int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                    int32_t* status, void* stream);
 
 /* ---- sampling from given uniforms ---------------------------------------------
- * One token per row of logits [rows, vocab] (DDT_F32 or DDT_BF16, row stride in elements), with
- * per-row temperature, top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off) and the uniform
- * u in [0, 1); top_k / top_p / min_p may be NULL (off for all rows).
+ * One token per row of logits [rows, vocab] (DDT_F32 or DDT_BF16, row stride in elements: at
+ * least vocab, or 0 for several draws from one row), with per-row temperature, top_k (<= 0:
+ * off), top_p (>= 1: off), min_p (<= 0: off) and the uniform u in [0, 1); top_k / top_p / min_p
+ * may be NULL (off for all rows).
  * With z_i = (x_i - max x) / temperature (0 where x_i is the maximum) the weight of token i is
  * the whole number floor(exp(z_i) * 2^40): sums of weights are exact, so a row's token does not
  * depend on the launch, the batch or the order of the sums.  Kept are the first tokens by (logit

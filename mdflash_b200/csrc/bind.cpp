@@ -170,7 +170,7 @@ Tensor paged_qk_norm_rope(const Tensor& qkv, const Tensor& q_norm_w, const Tenso
   } else {
     o = fresh({T, hq, d}, at::kBFloat16, idx);
   }
-  check(ddt_paged_qk_norm_rope(ptr(qkv), std::max(qkv.stride(0), width), T, hq, pool.heads, d,
+  check(ddt_paged_qk_norm_rope(ptr(qkv), T > 1 ? qkv.stride(0) : width, T, hq, pool.heads, d,
                                ptr(q_norm_w), ptr(k_norm_w), static_cast<float>(eps),
                                ptr(rope_table), ptr<int64_t>(slot_map), ptr(o), ptr(k_pages),
                                ptr(v_pages), pool.pages, pool.page, pool.page_stride,
@@ -237,7 +237,7 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& u, const T
   const Tensor o = out ? *out : fresh({rows}, at::kLong, idx);
   const Tensor lp = logprobs ? *logprobs : fresh({rows}, at::kFloat, idx);
   check(ddt_sample(ptr(logits), logits.scalar_type() == at::kFloat ? DDT_F32 : DDT_BF16, rows, vocab,
-                   std::max(logits.stride(0), vocab), ptr<float>(u), ptr<float>(temperature),
+                   rows > 1 ? logits.stride(0) : vocab, ptr<float>(u), ptr<float>(temperature),
                    ptr<int32_t>(top_k), ptr<float>(top_p), ptr<float>(min_p), ptr<int64_t>(o),
                    ptr<float>(lp), stream_of(idx)),
         "ddt_sample");

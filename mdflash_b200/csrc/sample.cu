@@ -1042,7 +1042,7 @@ extern "C" int ddt_sample(const void* logits, int dtype, int64_t rows, int64_t v
                           const int32_t* top_k, const float* top_p, const float* min_p,
                           int64_t* tokens, float* logprobs, void* stream) {
   if (dtype != DDT_F32 && dtype != DDT_BF16) return DDT_ERR_DTYPE;
-  if (rows < 0 || vocab <= 0 || row_stride < vocab) return DDT_ERR_INVALID;
+  if (rows < 0 || vocab <= 0 || (row_stride < vocab && row_stride != 0)) return DDT_ERR_INVALID;
   if (vocab >= (int64_t(1) << 22) || rows > 0x7fffffff / sample::kMaxCluster) return DDT_ERR_CAPACITY;
   if (rows == 0) return DDT_OK;
   if (!logits || !u || !temperature || !tokens) return DDT_ERR_INVALID;

@@ -979,10 +979,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
            top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
            min_p: torch.Tensor | None = None, out: torch.Tensor | None = None,
            logprobs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """ddt_sample: one token per row of logits [rows, vocab] (f32 or bf16) from the given
-    uniforms u f32 [rows], with per-row temperature f32, top_k i32, top_p f32 and min_p f32
-    (None: off).  Returns (tokens i64 [rows], logprobs f32 [rows]); -1 and -inf for a row
-    without a token to draw."""
+    """ddt_sample: one token per row of logits [rows, vocab] (f32 or bf16; one row expanded to
+    [rows, vocab] is read where it is) from the given uniforms u f32 [rows], with per-row
+    temperature f32, top_k i32, top_p f32 and min_p f32 (None: off).  Returns (tokens i64 [rows],
+    logprobs f32 [rows]); -1 and -inf for a row without a token to draw."""
     drawn = _lib.binding().sample(logits, u, temperature, top_k, top_p, min_p, out, logprobs)
     STATS.launches += 1
     return drawn

@@ -232,6 +232,24 @@ def test_paged_write_zero_rows_and_slots_outside(cuda_device):
     assert K.paged_qk_norm_rope(qkv[:0], w, w, words[:0], slots[:0], kp, vp).shape == (0, 1, D)
 
 
+def test_paged_write_refuses_rows_that_overlap(cuda_device):
+    """One projection row expanded to several tokens, or rows closer than their width, are
+    refused; the stride of a single row does not matter."""
+    kp, vp = (_pool(2, 1, 16, "heads_first", cuda_device) for _ in range(2))
+    w = torch.ones(D, dtype=torch.bfloat16, device=cuda_device)
+    words = _rope(torch.arange(3))[0].to(cuda_device)
+    slots = torch.arange(3, device=cuda_device)
+    one = torch.randn((1, 3 * D), device=cuda_device).to(torch.bfloat16)
+    for qkv in (one.expand(3, -1), torch.zeros(9 * D, dtype=torch.bfloat16, device=cuda_device)
+                .as_strided((3, 3 * D), (2 * D, 1))):
+        with pytest.raises(_lib.DDTreeError):
+            K.paged_qk_norm_rope(qkv, w, w, words, slots, kp, vp)
+    q = K.paged_qk_norm_rope(one, w, w, words[:1], slots[:1], kp, vp)
+    k, v = kp[0, :, 0].clone(), vp[0, :, 0].clone()
+    q2 = K.paged_qk_norm_rope(one.as_strided((1, 3 * D), (7, 1)), w, w, words[:1], slots[1:2], kp, vp)
+    assert torch.equal(q, q2) and torch.equal(kp[0, :, 1], k) and torch.equal(vp[0, :, 1], v)
+
+
 # ---- attention -------------------------------------------------------------------------------
 class _Case:
     """Requests with random K / V in a shuffled pool; whatever lies outside their rows is NaN,

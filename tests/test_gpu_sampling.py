@@ -202,6 +202,29 @@ def test_sample_does_not_depend_on_the_batch_or_strides(cuda_device):
         assert torch.equal(one[0], tok[r:r + 1]) and torch.equal(one[1], logp[r:r + 1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [9, 9001, 40960])
+def test_sample_several_draws_from_one_row(cuda_device, dtype, V):
+    """One row of logits expanded to many (stride 0), the last row of its storage: every draw is
+    the one of a copy of the row.  Rows that overlap in any other way are refused."""
+    g = torch.Generator().manual_seed(V)
+    rows = 37
+    x = (torch.randn((3, V), generator=g) * 3).to(dtype).to(cuda_device)
+    u = torch.rand(rows, generator=g).to(cuda_device)
+    temp = torch.full((rows,), 0.8, device=cuda_device)
+    k = torch.tensor([0, 40, 0] * 12 + [5], dtype=torch.int32, device=cuda_device)
+    p = torch.tensor([1.0, 0.9, 0.8] * 12 + [1.0], device=cuda_device)
+    wide = x[2].expand(rows, V)
+    assert wide.stride(0) == 0
+    tok, logp = K.sample(wide, u, temp, k, p)
+    tok2, logp2 = K.sample(wide.contiguous(), u, temp, k, p)
+    assert torch.equal(tok, tok2) and torch.equal(logp, logp2)
+    one = K.sample(x[2:], u[:1], temp[:1], k[:1], p[:1])
+    assert torch.equal(one[0], tok[:1]) and torch.equal(one[1], logp[:1])
+    with pytest.raises(_lib.DDTreeError):
+        K.sample(x.flatten().as_strided((4, V), (V // 2, 1)), u[:4], temp[:4])
+
+
 @pytest.mark.parametrize("k,p,mp", [(0, 1.0, 0.0), (6, 1.0, 0.0), (0, 0.8, 0.0), (0, 1.0, 0.2)])
 def test_sample_distribution(cuda_device, k, p, mp):
     """120k draws from 16 tokens: a chi-square test against the truncated softmax (at most 15
