@@ -3,6 +3,7 @@
 // host side (a 2 us kernel behind 13 us of checks and allocations in Python, per layer and step
 // of a server that does not record its step), which is why they have this binding beside the C
 // ABI's; what it calls is the C ABI.
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -77,6 +78,14 @@ void need_status(const Tensor& first, const Tensor& status) {
 }
 
 void* stream_of(int idx) { return c10::cuda::getCurrentCUDAStream(idx).stream(); }
+
+// The recording that the current stream of a device takes part in, or 0.
+uint64_t capture_id(int idx) {
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(idx).stream(), &status, &id));
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
 
 // (row stride, columns) of a block table i32 [requests, max_pages]
 std::pair<int64_t, int64_t> table_view(const Tensor& t, int64_t requests) {
@@ -247,6 +256,7 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& u, const T
 }  // namespace
 
 PYBIND11_MODULE(_bind, m) {
+  m.def("capture_id", &capture_id);
   m.def("page_tables", &page_tables);
   m.def("paged_qk_norm_rope", &paged_qk_norm_rope);
   m.def("paged_attention", &paged_attention);

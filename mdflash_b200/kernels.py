@@ -888,8 +888,7 @@ class PageStep:
 
 # These launches are shorter than their host side, so their checks, outputs and launch are one call
 # of the compiled binding (csrc/bind.cpp).  Their workspaces hold counters that have to be zero
-# between calls, so every stream has its own, and recorded calls one per lane (graphs that may
-# replay at the same time are recorded in different lanes).
+# between calls, so every stream has its own, and so has every stream of a recording.
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
@@ -903,18 +902,43 @@ def _paged_bytes() -> tuple[int, int]:
             lib.ddt_paged_attn_workspace_bytes(1 << 20, 1 << 20, 64, 1))
 
 
+# (device, name, lane, recording) -> the workspace of each of its streams
+_RECORDING: dict[tuple, dict[int, torch.Tensor]] = {}
+
+
+def _recorded_workspace(t: torch.Tensor, name: str, nbytes: int, recording: int) -> torch.Tensor:
+    """The workspace of a call that is being recorded.  A recording's first stream takes the one
+    of (device, lane)'s recorded calls, made beside the first eager call's own: memory allocated
+    during a recording would be zeroed by that graph's replays only.  Each further stream, whose
+    calls may replay beside the first one's, gets one of the graph's own memory and zeroes it in
+    every replay."""
+    idx = t.get_device()
+    first = WORKSPACES.find(idx, (name, "recorded"))
+    if first is None:
+        raise _lib.DDTreeError(f"{name}: call it once on this device and lane before recording it")
+    key = (idx, name, WORKSPACES.current_lane, recording)
+    streams = _RECORDING.get(key)
+    if streams is None:
+        # (a graph's pool keeps the memory for its replays; here it is needed while recording)
+        for old in [k for k in _RECORDING if k[:3] == key[:3]][:-4]:
+            del _RECORDING[old]
+        streams = _RECORDING[key] = {}
+    stream = _raw_stream(idx)
+    ws = streams.get(stream)
+    if ws is None:
+        ws = streams[stream] = torch.zeros(nbytes, dtype=torch.uint8, device=t.device) if streams \
+            else first
+    return ws
+
+
 def _stream_workspace(t: torch.Tensor, name: str, nbytes: int) -> torch.Tensor:
-    """The zeroed workspace of (t's device, lane, current stream), or, while a graph is recorded, of
-    (device, lane)'s recorded calls.  That one is made beside the first call's own: memory allocated
-    during a recording would be zeroed by that graph's replays only."""
+    """The zeroed workspace of (t's device, lane, current stream)."""
     idx = t.get_device()
     if idx < 0:
         _require_cuda(t)
-    if torch.cuda.is_current_stream_capturing():
-        ws = WORKSPACES.find(idx, (name, "recorded"))
-        if ws is None:
-            raise _lib.DDTreeError(f"{name}: call it once on this device and lane before recording it")
-        return ws
+    recording = _lib.binding().capture_id(idx)
+    if recording:
+        return _recorded_workspace(t, name, nbytes, recording)
     stream = _raw_stream(idx)
     ws = WORKSPACES.find(idx, (name, stream))
     if ws is None:

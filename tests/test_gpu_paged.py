@@ -517,6 +517,59 @@ def test_paged_attention_recorded_without_a_first_call_is_refused(cuda_device):
     c.check(out)
 
 
+@pytest.mark.parametrize("lane", [0, 5])
+def test_paged_kernels_recorded_on_parallel_branches(cuda_device, lane):
+    """One recording that forks into three streams and joins them again, each with attention calls
+    of cut units and page steps: branches that replay at once share no scratch.  Several replays
+    give what the calls give alone, and so does a second recording of the same branches."""
+    cases = [_Case(cuda_device, [5000, 3000], [1, 1], 32, 8, 16, seed=1),
+             _Case(cuda_device, [4000, 900], [1, 300], 32, 8, 16, seed=2),
+             _Case(cuda_device, [7000], [1], 32, 8, 16, seed=3)]
+    side = [torch.cuda.Stream() for _ in cases[1:]]
+    lens = [_i32(c.lens, cuda_device) for c in cases]
+    zero = [torch.zeros_like(n) for n in lens]
+    free, count = torch.arange(1000, dtype=torch.int32, device=cuda_device), _i32([1000], cuda_device)
+    outs = [[torch.zeros_like(c.q) for _ in range(6)] for c in cases]
+    steps = [[K.PageStep.allocate(cuda_device, len(c.lens), 9000) for _ in range(6)] for c in cases]
+    tables = [c.table.clone() for c in cases]
+
+    def branch(i):
+        for o, step in zip(outs[i], steps[i]):
+            cases[i].run(out=o)
+            K.page_tables(zero[i], lens[i], tables[i], free, count, 16, 9000, out=step)
+
+    with K.WORKSPACES.lane(lane):
+        alone = [c.run() for c in cases]
+        for i in range(3):
+            branch(i)
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                main = torch.cuda.current_stream()
+                for i, st in enumerate(side, 1):
+                    st.wait_stream(main)
+                    with torch.cuda.stream(st):
+                        branch(i)
+                branch(0)
+                for st in side:
+                    main.wait_stream(st)
+                cases[1].run(out=outs[1][0])
+            for _ in range(5):
+                for i in range(3):
+                    for o, step in zip(outs[i], steps[i]):
+                        o.fill_(7)
+                        step.slot_map.fill_(-5)
+                graph.replay()
+                torch.cuda.synchronize()
+                for i, c in enumerate(cases):
+                    assert all(torch.equal(o, alone[i]) for o in outs[i])
+                    for step in steps[i]:
+                        assert step.kv_lens.tolist() == c.lens
+                        assert int((step.slot_map >= 0).sum()) == sum(c.lens)
+    for i, c in enumerate(cases):
+        c.check(outs[i][0])
+
+
 @pytest.mark.parametrize("news", [[1, 1, 1, 1], [16, 3, 16, 1], [100, 1, 300, 64]])
 def test_paged_attention_recorded_once_serves_other_lengths(cuda_device, news):
     """One recorded launch, replayed after the lengths, tables and queries changed; launched on
