@@ -822,10 +822,12 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   // longest request, so the others are judged by their mean: where they are not 16 rows or
   // fewer, or too few to fill the SMs, this kernel takes all.  (Recorded graph, a 1000-token
   // chunk among 32 decoded tokens of 1k to 7k keys: 118 us on this kernel alone, 105 on both;
-  // among 3, where it takes all, 49.)
+  // among 3, where it takes all, 49.)  Groups of more than 16 heads have no room in that kernel's
+  // tile of 16 rows.
   const bool few = p.max_new * group <= kShortRows;
   const int64_t others = n_requests - 1, one_tile = 16 / group;
-  const bool both = !few && others * kv_heads >= kSms && n_tokens - p.max_new <= one_tile * others;
+  const bool both = !few && one_tile > 0 && others * kv_heads >= kSms &&
+                    n_tokens - p.max_new <= one_tile * others;
   CUtensorMap tm_q, tm_k, tm_v;
   const cuuint64_t kdims[4] = {kHeadDim, static_cast<cuuint64_t>(page_size),
                                static_cast<cuuint64_t>(kv_heads), static_cast<cuuint64_t>(n_pages)};

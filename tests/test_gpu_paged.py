@@ -424,6 +424,23 @@ def test_paged_attention_skips_requests_out_of_range(cuda_device):
         assert bool((out[16:16 + skip] == 3).all())
 
 
+@pytest.mark.parametrize("hq,hkv", [(17, 1), (32, 1), (64, 1), (128, 2)])
+@pytest.mark.parametrize("what", ["prompt_among_idle_places", "decodes_with_a_loose_bound"])
+def test_paged_attention_wide_groups_among_many_places(cuda_device, hq, hkv, what):
+    """More than 16 query heads per KV head in a batch of many places: the first prompt of an
+    otherwise idle server, and decoded tokens whose announced bound is the whole batch."""
+    places = 160
+    if what == "prompt_among_idle_places":
+        lens, news = [0] * places, [0] * places
+        lens[70], news[70] = 130, 100
+    else:
+        lens, news = [3 * i + 1 for i in range(places)], [1] * places
+    c = _Case(cuda_device, lens, news, hq, hkv, 16, seed=hq)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    c.check(c.run(max_new=c.cu[-1], status=status))
+    assert int(status.item()) == 0
+
+
 def test_paged_attention_rows_without_request_are_left(cuda_device):
     c = _Case(cuda_device, [70, 9], [3, 2], 8, 2, 16)
     q = torch.cat([c.q, c.q[:4]])
