@@ -492,7 +492,13 @@ int ddt_mask_to_bits(const void* mask, int dtype, int64_t n_nodes, int64_t row_s
  * rows outside [0, n_tokens], kv_lens[r] outside [0, max_pages * page_size]) is skipped and
  * *status gets DDT_STATUS_PAGED_RANGE.  head_dim 128, q_heads a multiple of kv_heads, at most
  * 64 query heads per KV head.
- * The workspace (ddt_paged_attn_workspace_bytes) must be zero-filled before its first use. */
+ * The workspace (ddt_paged_attn_workspace_bytes) must be zero-filled before its first use; every
+ * launch leaves its counters zero, one whose waits ran out (DDT_ERR_TIMEOUT) too.
+ *
+ * ddt_paged_attn_wait_check: like ddt_paged_attn, with every wait bounded by timeout_ns (100 us ..
+ * 2 s, the limit of ddt_paged_attn) and no load issued by the CTAs from first_cta on, so that
+ * their waits run out: the launch returns, *status (device i32, not NULL) is set where any of
+ * them had work, and the rows that it did not finish are not defined. */
 #define DDT_MAX_PAGED_REQUESTS 2048
 #define DDT_STATUS_PAGES 16
 #define DDT_STATUS_PAGED_RANGE 32
@@ -521,6 +527,16 @@ int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                    int64_t head_dim, float scale, void* out, int64_t o_token_stride,
                    int64_t o_head_stride, void* workspace, size_t workspace_bytes,
                    int32_t* status, void* stream);
+int ddt_paged_attn_wait_check(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const void* k_pages, const void* v_pages, int64_t n_pages,
+                              int64_t page_size, int64_t page_stride, int64_t head_stride,
+                              int64_t row_stride, const int32_t* block_table, int64_t table_stride,
+                              int64_t max_pages, const int32_t* cu_new, const int32_t* kv_lens,
+                              int64_t n_requests, int64_t n_tokens, int64_t max_new,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale,
+                              void* out, int64_t o_token_stride, int64_t o_head_stride,
+                              void* workspace, size_t workspace_bytes, int32_t* status,
+                              int64_t first_cta, uint64_t timeout_ns, void* stream);
 
 /* ---- sampling from given uniforms ---------------------------------------------
  * One token per row of logits [rows, vocab] (DDT_F32 or DDT_BF16, row stride in elements: at

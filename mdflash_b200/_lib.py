@@ -100,6 +100,9 @@ SIGNATURES = {
     "ddt_paged_attn_workspace_bytes": (_S, [_I, _I, _I, _I]),
     "ddt_paged_attn": (_i, [_P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I,
                             _I, _I, _I, _F, _P, _I, _I, _P, _S, _P, _P]),
+    "ddt_paged_attn_wait_check": (_i, [_P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I,
+                                       _I, _I, _I, _I, _I, _F, _P, _I, _I, _P, _S, _P, _I,
+                                       ctypes.c_uint64, _P]),
     "ddt_sample": (_i, [_P, _i, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 

@@ -11,6 +11,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "ddtree_b200.h"
 
@@ -188,10 +189,12 @@ Tensor paged_qk_norm_rope(const Tensor& qkv, const Tensor& q_norm_w, const Tenso
   return o;
 }
 
+// With wait_check (first CTA without loads, limit of the waits in ns): ddt_paged_attn_wait_check.
+using WaitCheck = std::optional<std::pair<int64_t, uint64_t>>;
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
                        const Tensor& block_table, const Tensor& cu_new, const Tensor& kv_lens,
                        int64_t max_new, std::optional<double> scale, const MaybeTensor& out,
-                       const Tensor& status, const Tensor& workspace) {
+                       const Tensor& status, const Tensor& workspace, const WaitCheck& wait_check) {
   const int idx = device_of(q, k_pages, v_pages, block_table, cu_new, kv_lens);
   const Pool pool(k_pages, v_pages);
   if (q.dim() != 3 || q.scalar_type() != at::kBFloat16 || q.stride(2) != 1)
@@ -200,7 +203,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   if (d != pool.dim) refuse("q and the pages differ in head_dim");
   need(kv_lens, at::kInt, {R}, "kv_lens");
   need(cu_new, at::kInt, {R + 1}, "cu_new");
-  const auto [stride, cols] = table_view(block_table, R);
+  const std::pair<int64_t, int64_t> table = table_view(block_table, R);
   need_status(q, status);
   Tensor o;
   if (out) {
@@ -211,14 +214,19 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   } else {
     o = fresh({T, hq, d}, at::kBFloat16, idx);
   }
-  check(ddt_paged_attn(ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), pool.pages,
-                       pool.page, pool.page_stride, pool.head_stride, pool.row_stride,
-                       ptr<int32_t>(block_table), stride, cols, ptr<int32_t>(cu_new),
-                       ptr<int32_t>(kv_lens), R, T, max_new, hq, pool.heads, d,
-                       static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d))),
-                       ptr(o), o.stride(0), o.stride(1), ptr(workspace), workspace.numel(),
-                       ptr<int32_t>(status), stream_of(idx)),
-        "ddt_paged_attn");
+  const auto call = [&](auto entry, const char* name, auto... wait) {
+    check(entry(ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), pool.pages, pool.page,
+                pool.page_stride, pool.head_stride, pool.row_stride, ptr<int32_t>(block_table),
+                table.first, table.second, ptr<int32_t>(cu_new), ptr<int32_t>(kv_lens), R, T, max_new, hq, pool.heads, d,
+                static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d))), ptr(o),
+                o.stride(0), o.stride(1), ptr(workspace), workspace.numel(), ptr<int32_t>(status),
+                wait..., stream_of(idx)),
+          name);
+  };
+  if (wait_check)
+    call(ddt_paged_attn_wait_check, "ddt_paged_attn_wait_check", wait_check->first, wait_check->second);
+  else
+    call(ddt_paged_attn, "ddt_paged_attn");
   return o;
 }
 

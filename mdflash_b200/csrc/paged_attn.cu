@@ -192,7 +192,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           pg = p.block_table[it.r * p.table_stride + (key >> p.page_shift)];
         return pg >= 0 && pg < p.n_pages ? pg : static_cast<int>(p.n_pages);
       };
-      while (ok && next()) {
+      while (ok && blockIdx.x < p.withhold_from && next()) {
         const int t0 = it.t0, nt = it.nt;
         if (nt == 0) continue;
         int pg_next = page_id(t0);
@@ -750,32 +750,15 @@ constexpr size_t kWorkspace = kPartO + kPartMl + kSms * sizeof(int4);
 // The long kernel's area comes after the short one's, whose counters have to stay zero.
 inline size_t workspace_bytes() { return (short_workspace_bytes() + 255) / 256 * 256 + kWorkspace; }
 
-}  // namespace paged_attn
-}  // namespace ddt
-
-using namespace ddt;
-
-extern "C" size_t ddt_paged_attn_workspace_bytes(int64_t n_tokens, int64_t max_new,
-                                                 int64_t q_heads, int64_t kv_heads) {
-  (void)n_tokens;
-  (void)max_new;
-  (void)q_heads;
-  (void)kv_heads;
-  // how units are cut depends on device-side lengths: one size for all calls
-  return paged_attn::workspace_bytes();
-}
-
-extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                              const void* k_pages, const void* v_pages, int64_t n_pages,
-                              int64_t page_size, int64_t page_stride, int64_t head_stride,
-                              int64_t row_stride, const int32_t* block_table, int64_t table_stride,
-                              int64_t max_pages, const int32_t* cu_new, const int32_t* kv_lens,
-                              int64_t n_requests, int64_t n_tokens, int64_t max_new,
-                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale,
-                              void* out, int64_t o_token_stride, int64_t o_head_stride,
-                              void* workspace, size_t workspace_bytes, int32_t* status,
-                              void* stream) {
-  using namespace paged_attn;
+// A call of either entry point: timeout_ns bounds every wait, CTAs from withhold_from on issue no
+// load (the check of the waits).
+int call(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_pages,
+         const void* v_pages, int64_t n_pages, int64_t page_size, int64_t page_stride,
+         int64_t head_stride, int64_t row_stride, const int32_t* block_table, int64_t table_stride,
+         int64_t max_pages, const int32_t* cu_new, const int32_t* kv_lens, int64_t n_requests,
+         int64_t n_tokens, int64_t max_new, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+         float scale, void* out, int64_t o_token_stride, int64_t o_head_stride, void* workspace,
+         size_t ws_bytes, int32_t* status, void* stream, uint64_t timeout_ns, unsigned withhold_from) {
   if (n_requests <= 0 || n_tokens < 0 || max_new < 0 || q_heads <= 0 || kv_heads <= 0 ||
       q_heads % kv_heads || n_pages <= 0 || max_pages <= 0 || table_stride < max_pages ||
       !(scale >= 0.f))
@@ -792,7 +775,7 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
       q_token_stride % 8 || q_head_stride % 8 || page_stride % 8 || head_stride % 8 ||
       row_stride % 8 || o_token_stride % 8 || o_head_stride % 8)
     return DDT_ERR_ALIGN;
-  if (!workspace || workspace_bytes < paged_attn::workspace_bytes()) return DDT_ERR_WORKSPACE;
+  if (!workspace || ws_bytes < workspace_bytes()) return DDT_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return DDT_ERR_ALIGN;
   const int64_t group = q_heads / kv_heads;
   Params p;
@@ -815,7 +798,8 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   p.o_token_stride = o_token_stride;
   p.o_head_stride = o_head_stride;
   p.status = status;
-  p.timeout_ns = kTimeoutNs;
+  p.timeout_ns = timeout_ns;
+  p.withhold_from = withhold_from;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Which kernel takes which request: few rows go to the short one, the rest to this one, and
   // a batch of long chunks with single tokens between them to both.  The host knows only the
@@ -874,4 +858,58 @@ extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_h
   return launch_early(paged_merge_kernel,
                       dim3(kSms, kUnitRows / 32 * (kHeadDim / kMergeDims) / kMergeWarps),
                       dim3(kMergeWarps * 32), 0, st, 0, p);
+}
+
+}  // namespace paged_attn
+}  // namespace ddt
+
+using namespace ddt;
+
+extern "C" size_t ddt_paged_attn_workspace_bytes(int64_t n_tokens, int64_t max_new,
+                                                 int64_t q_heads, int64_t kv_heads) {
+  (void)n_tokens;
+  (void)max_new;
+  (void)q_heads;
+  (void)kv_heads;
+  // how units are cut depends on device-side lengths: one size for all calls
+  return paged_attn::workspace_bytes();
+}
+
+extern "C" int ddt_paged_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const void* k_pages, const void* v_pages, int64_t n_pages,
+                              int64_t page_size, int64_t page_stride, int64_t head_stride,
+                              int64_t row_stride, const int32_t* block_table, int64_t table_stride,
+                              int64_t max_pages, const int32_t* cu_new, const int32_t* kv_lens,
+                              int64_t n_requests, int64_t n_tokens, int64_t max_new,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale,
+                              void* out, int64_t o_token_stride, int64_t o_head_stride,
+                              void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return paged_attn::call(q, q_token_stride, q_head_stride, k_pages, v_pages, n_pages, page_size,
+                          page_stride, head_stride, row_stride, block_table, table_stride,
+                          max_pages, cu_new, kv_lens, n_requests, n_tokens, max_new, q_heads,
+                          kv_heads, head_dim, scale, out, o_token_stride, o_head_stride, workspace,
+                          workspace_bytes, status, stream, paged_attn::kTimeoutNs, ~0u);
+}
+
+extern "C" int ddt_paged_attn_wait_check(const void* q, int64_t q_token_stride,
+                                         int64_t q_head_stride, const void* k_pages,
+                                         const void* v_pages, int64_t n_pages, int64_t page_size,
+                                         int64_t page_stride, int64_t head_stride,
+                                         int64_t row_stride, const int32_t* block_table,
+                                         int64_t table_stride, int64_t max_pages,
+                                         const int32_t* cu_new, const int32_t* kv_lens,
+                                         int64_t n_requests, int64_t n_tokens, int64_t max_new,
+                                         int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                         float scale, void* out, int64_t o_token_stride,
+                                         int64_t o_head_stride, void* workspace,
+                                         size_t workspace_bytes, int32_t* status, int64_t first_cta,
+                                         uint64_t timeout_ns, void* stream) {
+  if (!status || first_cta < 0 || timeout_ns < 100000ull || timeout_ns > paged_attn::kTimeoutNs)
+    return DDT_ERR_INVALID;
+  const unsigned first = first_cta < 0x7fffffff ? static_cast<unsigned>(first_cta) : 0x7fffffffu;
+  return paged_attn::call(q, q_token_stride, q_head_stride, k_pages, v_pages, n_pages, page_size,
+                          page_stride, head_stride, row_stride, block_table, table_stride,
+                          max_pages, cu_new, kv_lens, n_requests, n_tokens, max_new, q_heads,
+                          kv_heads, head_dim, scale, out, o_token_stride, o_head_stride, workspace,
+                          workspace_bytes, status, stream, timeout_ns, first);
 }

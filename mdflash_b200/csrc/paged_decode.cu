@@ -22,7 +22,8 @@
 // HBM.  One request of 1000 keys takes 9.7 us, two thirds of it dependent reads (lengths, page
 // ids, K, the parts).
 // Units are cut over the CTAs as in paged_sched.cuh; the CTA that brings a cut unit's last part
-// merges all of them, in the order of the CTAs, so the result does not depend on which it is.
+// merges all of them, in the order of the CTAs, so the result does not depend on which it is, and
+// sets the unit's counter back to zero.
 #include "paged_sched.cuh"
 
 namespace ddt {
@@ -235,7 +236,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         ++turn;
       }
     };
-    while (ok && next()) {
+    while (ok && blockIdx.x < p.withhold_from && next()) {
       const int t0 = it.t0, nt = it.nt;
       if (nt == 0) continue;
       const int qb = n_item & 1;
@@ -290,7 +291,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       ++turn;
     }
   };
+  // (after a failed wait the walk goes on without work: this CTA's parts are still counted, so
+  // that the counters of cut units end at zero)
   while (next()) {
+    const bool works = ok;  // the same in all four warps
     const int t0 = it.t0, nt = it.nt, len = it.len;
     const int rows = it.n_tok * p.group;
     float o[kM][4][4], m[kM][2], l[kM][2];
@@ -310,9 +314,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         for (int e = 0; e < 4; ++e) o[a][n][e] = 0.f;
     }
     const uint32_t sQ = base + L::kQ + (n_item & 1) * 2 * L::kQHalf;
-    if (nt > 0)
+    if (works && nt > 0)
       ok = tc::mbar_wait_warp(&bars.q_full[n_item & 1], (n_item >> 1) & 1, abort_flag, p.timeout_ns);
-    for (int j = 0; j < nt; ++j) {
+    for (int j = 0; works && j < nt; ++j) {
       const int key0 = (t0 + j) * kKeys;
       // 1. S of this warp's 16 keys
       ok = ok && tc::mbar_wait_warp(&bars.full[buf], turn & 1, abort_flag, p.timeout_ns);
@@ -436,10 +440,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         l[a][h] += __shfl_xor_sync(DDT_FULL_MASK, l[a][h], 2);
         if (ok && t4 == 0) s_max[(a * 16 + h * 8 + g) * 4 + warp] = l[a][h];
       }
-    if (!tc::named_sync_and(1, kConsumers * 32, ok)) {
-      ok = false;
-      break;
-    }
+    ok = tc::named_sync_and(1, kConsumers * 32, ok);
+    if (!ok && lane == 0) *abort_flag = 1;  // the producer's waits end too
     if (nt > 0) ++n_item;
 #pragma unroll
     for (int a = 0; a < kM; ++a)
@@ -449,7 +451,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const float4 w = *reinterpret_cast<const float4*>(&s_max[r * 4]);
         const float sum = (w.x + w.y) + (w.z + w.w);
         if (r >= rows) continue;
-        if (it.slot < 0) {
+        if (!ok) {  // a part without weight
+          if (it.slot >= 0 && warp == 0 && t4 == 0)
+            *reinterpret_cast<float2*>(p.ml_part +
+                                       (static_cast<long long>(it.slot) * kShortRows + r) * 2) =
+                make_float2(-INFINITY, 0.f);
+        } else if (it.slot < 0) {
           const float inv = sum > 0.f ? 1.f / sum : 0.f;
           const int tok = r / p.group;
           __nv_bfloat16* dst = p.out + (it.tok0 + tok) * p.o_token_stride +

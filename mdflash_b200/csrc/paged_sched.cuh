@@ -47,6 +47,7 @@ struct Params {
   unsigned int* arrived;  // [CTAs]: parts written of the unit that starts in this CTA
   int32_t* status;
   unsigned long long timeout_ns;
+  unsigned int withhold_from;  // check of the waits: CTAs from this one on issue no load
 };
 
 // First query row, new tokens and key count of request r; no tokens where another launch takes

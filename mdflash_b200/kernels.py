@@ -18,7 +18,8 @@ __all__ = [
     "anc_words_for", "TreeBatch", "topk_tree_batched", "KvBatch", "accept_compact_batched",
     "attention_status", "check_status", "tree_attention_wait_check",
     "sample_chains", "chain_tree", "lm_head_argmax",
-    "PageStep", "page_tables", "paged_qk_norm_rope", "paged_attention", "sample",
+    "PageStep", "page_tables", "paged_qk_norm_rope", "paged_attention",
+    "paged_attention_wait_check", "sample",
 ]
 
 
@@ -994,7 +995,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ws = _stream_workspace(q, "paged_attn", _paged_bytes()[1])
     o = _lib.binding().paged_attention(
         q, k_pages, v_pages, block_table, cu_new, kv_lens, max_new, scale, out,
-        attention_status(q.device) if status is None else status, ws)
+        attention_status(q.device) if status is None else status, ws, None)
+    STATS.launches += 1
+    return o
+
+
+def paged_attention_wait_check(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                               block_table: torch.Tensor, cu_new: torch.Tensor,
+                               kv_lens: torch.Tensor, max_new: int, first_cta: int,
+                               timeout_ns: int, status: torch.Tensor) -> torch.Tensor:
+    """ddt_paged_attn_wait_check: one paged_attention whose CTAs from first_cta on withhold their
+    loads, so that their waits run out after timeout_ns; returns the output buffer, unfinished.
+    The caller reads `status` afterwards."""
+    ws = _stream_workspace(q, "paged_attn", _paged_bytes()[1])
+    o = _lib.binding().paged_attention(q, k_pages, v_pages, block_table, cu_new, kv_lens, max_new,
+                                       None, None, status, ws, (first_cta, timeout_ns))
     STATS.launches += 1
     return o
 

@@ -497,6 +497,29 @@ def test_paged_kernels_on_two_streams_at_once(cuda_device):
             assert int((st.slot_map >= 0).sum()) == sum(c.lens)
 
 
+@pytest.mark.parametrize("first_cta", [0, 5, 60, 120])
+@pytest.mark.parametrize("name", ["long_decode", "cut_blocks", "prompt_chunks", "chunk_among_30"])
+def test_paged_attention_wait_timeout_leaves_no_trace(cuda_device, name, first_cta):
+    """Every wait of the attention kernels is bounded.  The CTAs from first_cta on withhold their
+    loads, so that the waits in them run out (after 2 ms here): the launch returns and sets the
+    status word, and the calls after it on the same workspace are right, although units cut between
+    these CTAs and the others were left half done."""
+    lens, news, hq, hkv, page = ([9000, 7000], [5, 5], 16, 4, 16) if name == "cut_blocks" else ATTN[name]
+    c, d = (_Case(cuda_device, lens, news, hq, hkv, page, seed=s, vmean=m)
+            for s, m in ((len(name), 0.0), (1, 3.0)))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    K.paged_attention_wait_check(d.q, d.k_pages, d.v_pages, d.table, d.cu_new, d.kv_lens, max(news),
+                                 first_cta, 2_000_000, status)
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.DDTreeError, match="bounded device wait expired"):
+        K.check_status(status, "ddt_paged_attn")
+    outs = [c.run(status=status) for _ in range(4)]
+    torch.cuda.synchronize()
+    K.check_status(status, "ddt_paged_attn")
+    c.check(outs[0])
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 def test_paged_attention_mixed_batch_recorded(cuda_device):
     """Both kernels and the merge in a recorded graph, on a side stream, replayed back to back."""
     lens, news, hq, hkv, page = ATTN["chunk_among_30"]

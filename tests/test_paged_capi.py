@@ -60,6 +60,15 @@ def test_paged_attention_refusals(change, code):
     assert _call("ddt_paged_attn", ATTN, ATTN_OK, **change) == code
 
 
+@pytest.mark.parametrize("change,code", [
+    (dict(limit=99_999), -1), (dict(limit=2_000_000_001), -1), (dict(first=-1), -1),
+    (dict(status=None), -1), (dict(hq=30), -1), (dict(page=48), -2), (dict(q=ODD), -4),
+    (dict(maxn=0), 0)])
+def test_paged_attention_wait_check_refusals(change, code):
+    order = ATTN.replace("stream", "first limit stream")
+    assert _call("ddt_paged_attn_wait_check", order, dict(ATTN_OK, first=0, limit=10 ** 6), **change) == code
+
+
 SAMPLE = "x dtype rows vocab rs u temp k p mp tok logp stream"
 SAMPLE_OK = dict(x=P, dtype=1, rows=2, vocab=100, rs=100, u=P, temp=P, k=P, p=P, mp=P, tok=P, logp=P, stream=None)
 
