@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib
 from . import kernels as K
 
 
@@ -72,7 +73,8 @@ def paged_generate(runner, prompts: list[torch.Tensor], max_new_tokens: int,
     token of every decoding request and fills up to chunk_tokens with the next chunks of the
     prompts; the uniforms come from ``generator`` (torch's default one without it), one per
     drawn token.  n_pages: the pool's size (default: what all requests need at once; with fewer
-    a prompt waits until its pages are free)."""
+    a prompt waits until its pages are free).
+    Raises DDTreeError for a row of logits without a token to draw (all NaN or -inf)."""
     dev = runner.device
     if chunk_tokens < len(prompts):
         raise ValueError("chunk_tokens must leave every request a token")
@@ -135,6 +137,9 @@ def paged_generate(runner, prompts: list[torch.Tensor], max_new_tokens: int,
             u = torch.rand(len(drawn), device=dev, generator=generator)
             tokens, _ = K.sample(logits, u, **rules(len(drawn)))
             for r, t in zip(drawn, tokens.tolist()):
+                if t < 0:
+                    raise _lib.DDTreeError(f"request {r}: no token to draw after {len(answer[r])} "
+                                           "(its logits are all NaN or -inf)")
                 answer[r].append(t)
                 ended[r] = len(answer[r]) >= max_new_tokens or t in stop
         cache.check()

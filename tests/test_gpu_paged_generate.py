@@ -137,6 +137,32 @@ def test_paged_generate_samples_reproducibly_and_stops(cuda_device, runner):
     assert first <= 7
 
 
+@pytest.mark.parametrize("bad", [float("nan"), -float("inf")])
+@pytest.mark.parametrize("step", [0, 2])
+def test_paged_generate_reports_a_row_without_a_token(cuda_device, runner, bad, step):
+    """Logits of one request that hold nothing to draw, in the first step or in a later one, raise
+    an error on the host; the row's -1 is not fed to the embedding."""
+
+    class Broken:
+        steps = 0
+
+        def __getattr__(self, name):
+            return getattr(runner, name)
+
+        def forward_paged(self, ids, *args):
+            assert int(ids.min()) >= 0
+            logits = runner.forward_paged(ids, *args)
+            if self.steps == step:
+                logits[1] = bad
+            self.steps += 1
+            return logits
+
+    broken = Broken()
+    with pytest.raises(_lib.DDTreeError, match="request 1: no token to draw"):
+        paged_generate(broken, [torch.arange(9), torch.arange(40)], 6)
+    assert broken.steps == step + 1
+
+
 def test_recorded_decode_step_serves_growing_requests(cuda_device, runner):
     """Page tables, forward and sampling of a decode step recorded in one graph, replayed while
     the requests grow across pages: the tokens of the eager loop."""
