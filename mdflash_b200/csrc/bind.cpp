@@ -2,8 +2,10 @@
 // output tensors and the launch in one call from Python.  These launches are shorter than their
 // host side (a 2 us kernel behind 13 us of checks and allocations in Python, per layer and step
 // of a server that does not record its step), which is why they have this binding beside the C
-// ABI's; what it calls is the C ABI.
+// ABI's; what it calls is the C ABI, on the tensors' device and its current stream, whichever
+// device is the current one.
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -116,6 +118,7 @@ Step page_tables(const Tensor& old_lens, const Tensor& new_lens, const Tensor& b
                  int64_t max_tokens, const std::optional<Step>& out, const Tensor& status,
                  const Tensor& workspace) {
   const int idx = device_of(old_lens, new_lens, block_table, free_pages, free_count);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(idx));
   const int64_t R = old_lens.numel();
   need(old_lens, at::kInt, {R}, "old_lens");
   need(new_lens, at::kInt, {R}, "new_lens");
@@ -157,6 +160,7 @@ Tensor paged_qk_norm_rope(const Tensor& qkv, const Tensor& q_norm_w, const Tenso
                           const Tensor& rope_table, const Tensor& slot_map, const Tensor& k_pages,
                           const Tensor& v_pages, double eps, const MaybeTensor& out) {
   const int idx = device_of(qkv, q_norm_w, k_norm_w, rope_table, slot_map, k_pages, v_pages);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(idx));
   const Pool pool(k_pages, v_pages);
   const int64_t d = pool.dim;
   if (qkv.dim() != 2 || qkv.scalar_type() != at::kBFloat16 || qkv.stride(1) != 1 || d == 0 ||
@@ -196,6 +200,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                        int64_t max_new, std::optional<double> scale, const MaybeTensor& out,
                        const Tensor& status, const Tensor& workspace, const WaitCheck& wait_check) {
   const int idx = device_of(q, k_pages, v_pages, block_table, cu_new, kv_lens);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(idx));
   const Pool pool(k_pages, v_pages);
   if (q.dim() != 3 || q.scalar_type() != at::kBFloat16 || q.stride(2) != 1)
     refuse("q must be bf16 [tokens, q_heads, head_dim] with contiguous rows");
@@ -235,6 +240,7 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& u, const T
                                   const MaybeTensor& min_p, const MaybeTensor& out,
                                   const MaybeTensor& logprobs) {
   const int idx = device_of(logits, u, temperature);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(idx));
   if (logits.dim() != 2 || logits.stride(1) != 1)
     refuse("logits must be [rows, vocab] with unit stride");
   const int64_t rows = logits.size(0), vocab = logits.size(1);

@@ -215,6 +215,9 @@ class Qwen3VerifyRunner:
         layer writes its K/V rows into the pages and attends over them.  Returns the logits
         [len(rows), V] of the given rows (i64, device; None: all of them).  No counterpart in
         the reference, whose prefill and decode run on one contiguous cache per request."""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.forward_paged(ids, cache, step, max_new, rows, status)
         lib = _lib.load()
         st = self._stream()
         n = ids.numel()

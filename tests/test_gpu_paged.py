@@ -757,6 +757,35 @@ def test_paged_calls_recorded_after_other_work(cuda_device):
         assert torch.equal(t, token) and torch.equal(lp, logprob)
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_paged_calls_run_on_the_tensors_device():
+    """Tensors of a device that is not the current one: every call launches there, on that device's
+    current stream, eager and recorded."""
+    dev = torch.device("cuda:1")
+    with torch.cuda.device(0):
+        assert _run_tables(dev, [10, 20], [60, 12], 16, 8, 9, 64)
+        c = _Case(dev, [900, 70], [1, 40], 16, 4, 16)
+        c.check(c.run())
+        out = torch.zeros_like(c.q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.device(dev), torch.cuda.graph(graph):
+            with torch.cuda.device(0):
+                c.run(out=out)
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        c.check(out)
+        x = torch.randn((3, 50), device=dev)
+        tok, _ = K.sample(x, torch.rand(3, device=dev), torch.zeros(3, device=dev))
+        assert torch.equal(tok, x.argmax(-1))
+        w = torch.ones(D, dtype=torch.bfloat16, device=dev)
+        kp, vp = (_pool(2, 1, 16, "heads_first", dev) for _ in range(2))
+        qkv = torch.randn((2, 3 * D), device=dev).to(torch.bfloat16)
+        K.paged_qk_norm_rope(qkv, w, w, _rope(torch.arange(2))[0].to(dev),
+                             torch.arange(2, device=dev), kp, vp)
+        assert torch.equal(vp[0, 0, :2], qkv[:, 2 * D:])
+        assert torch.cuda.current_device() == 0
+
+
 def test_page_step_outputs_are_ordinary_tensors(cuda_device):
     """They share one allocation: each keeps it alive, and views, copies and torch operations see
     only its own elements."""
