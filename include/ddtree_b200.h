@@ -490,8 +490,9 @@ int ddt_mask_to_bits(const void* mask, int dtype, int64_t n_nodes, int64_t row_s
  * kv_lens[r] of a page may hold anything; rows below it must be finite.  max_new bounds n_r
  * (it picks the kernel).  A request whose lengths are out of range (n_r outside [0, max_new],
  * rows outside [0, n_tokens], kv_lens[r] outside [0, max_pages * page_size]) is skipped and
- * *status gets DDT_STATUS_PAGED_RANGE.  head_dim 128, q_heads a multiple of kv_heads, at most
- * 64 query heads per KV head.
+ * *status gets DDT_STATUS_PAGED_RANGE.  It gets it too where the table names a page outside the
+ * pool for a row below kv_lens[r]; that page is read as zeros.  head_dim 128, q_heads a multiple
+ * of kv_heads, at most 64 query heads per KV head.
  * The workspace (ddt_paged_attn_workspace_bytes) must be zero-filled before its first use; every
  * launch leaves its counters zero, one whose waits ran out (DDT_ERR_TIMEOUT) too.
  *

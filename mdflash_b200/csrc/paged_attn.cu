@@ -187,10 +187,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // page of this lane's box in key tile t, or n_pages (zeros) past the request's pages
       auto page_id = [&](int t) -> int {
         const long long key = static_cast<long long>(t) * kBlockN + box_row;
-        int pg = -1;
-        if (issues && key < it.len)
-          pg = p.block_table[it.r * p.table_stride + (key >> p.page_shift)];
-        return pg >= 0 && pg < p.n_pages ? pg : static_cast<int>(p.n_pages);
+        return issues && key < it.len ? page_of(p, it.r, key) : static_cast<int>(p.n_pages);
       };
       while (ok && blockIdx.x < p.withhold_from && next()) {
         const int t0 = it.t0, nt = it.nt;

@@ -216,10 +216,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     // page of this lane's box in key tile t, or n_pages (zeros) past the request's pages
     auto page_id = [&](int t) -> int {
       const int key = t * kKeys + box_row;
-      int pg = -1;
-      if (issues && key < it.len)
-        pg = p.block_table[it.r * p.table_stride + (key >> p.page_shift)];
-      return pg >= 0 && pg < p.n_pages ? pg : static_cast<int>(p.n_pages);
+      return issues && key < it.len ? page_of(p, it.r, key) : static_cast<int>(p.n_pages);
     };
     auto fill = [&](const CUtensorMap* map, int row, int pg) {
       if (used >= static_cast<uint32_t>(bufs) &&

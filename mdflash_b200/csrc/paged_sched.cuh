@@ -68,6 +68,15 @@ __device__ __forceinline__ Request request(const Params& p, int r) {
   return q;
 }
 
+// The page of request r that holds key `key`, or n_pages, from where the tensor maps read zeros (and
+// the status bit), where the table names no page of the pool.
+__device__ __forceinline__ int page_of(const Params& p, int r, long long key) {
+  const int page = p.block_table[r * p.table_stride + (key >> p.page_shift)];
+  if (page >= 0 && page < p.n_pages) return page;
+  if (p.status) atomicOr(p.status, DDT_STATUS_PAGED_RANGE);
+  return static_cast<int>(p.n_pages);
+}
+
 struct Item {
   int h, r;
   int tok0, n_tok;  // query rows of the unit: [tok0, tok0 + n_tok), all heads of the group

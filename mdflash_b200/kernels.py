@@ -126,7 +126,8 @@ STATUS_LAYOUT = 2       # a batched compaction met a head stride it cannot move
 STATUS_PAST_RANGE = 4   # a device-side prefix length was outside [0, planned maximum]
 STATUS_LOG_FULL = 8     # a decode-loop round found its output or length log full
 STATUS_PAGES = 16       # a page-table step was refused (pool exhausted or a bad length)
-STATUS_PAGED_RANGE = 32  # paged attention skipped a request whose lengths are out of range
+# paged attention skipped a request whose lengths are out of range, or met a page outside the pool
+STATUS_PAGED_RANGE = 32
 
 
 def check_status(status: torch.Tensor, what: str = "ddt_tree_attn") -> None:

@@ -450,6 +450,25 @@ def test_paged_attention_rows_without_request_are_left(cuda_device):
     assert bool((out[5:] == 3).all())
 
 
+@pytest.mark.parametrize("name", ["decode_mix", "blocks_of_16", "prompt_chunks"])
+@pytest.mark.parametrize("wrong", [-1, "past_the_pool", 1 << 30])
+def test_paged_attention_reports_pages_outside_the_pool(cuda_device, name, wrong):
+    """A table entry inside a request's length that names no page of the pool is reported; the
+    other requests are computed."""
+    lens, news, hq, hkv, page = ATTN[name]
+    c = _Case(cuda_device, lens, news, hq, hkv, page, seed=7)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    right = c.run(status=status)
+    assert int(status.item()) == 0
+    c.table[1, lens[1] // page // 2] = c.k_pages.shape[0] if wrong == "past_the_pool" else wrong
+    out = c.run(status=status)
+    assert int(status.item()) == K.STATUS_PAGED_RANGE
+    with pytest.raises(_lib.DDTreeError, match="paged request out of range"):
+        K.check_status(status, "ddt_paged_attn")
+    a, b = c.cu[1], c.cu[2]
+    c.check(torch.cat([out[:a], right[a:b], out[b:]]))
+
+
 def test_paged_attention_far_pages(cuda_device):
     """Page offsets beyond 2^32 elements: the rows of a small cache moved to the end of a pool of
     140,000 pages with 32,768 elements each."""
