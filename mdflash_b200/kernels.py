@@ -934,7 +934,9 @@ def _recorded_workspace(t: torch.Tensor, name: str, nbytes: int, recording: int)
 
 
 def _stream_workspace(t: torch.Tensor, name: str, nbytes: int) -> torch.Tensor:
-    """The zeroed workspace of (t's device, lane, current stream)."""
+    """The zeroed workspace of (t's device, lane, current stream).  The first one is made with the
+    device's default status word: one made during a recording would be zeroed by every replay,
+    with what others had reported in it."""
     idx = t.get_device()
     if idx < 0:
         _require_cuda(t)
@@ -944,6 +946,7 @@ def _stream_workspace(t: torch.Tensor, name: str, nbytes: int) -> torch.Tensor:
     stream = _raw_stream(idx)
     ws = WORKSPACES.find(idx, (name, stream))
     if ws is None:
+        attention_status(t.device)
         WORKSPACES.get(t.device, (name, "recorded"), nbytes)
         ws = WORKSPACES.get(t.device, (name, stream), nbytes)
     return ws

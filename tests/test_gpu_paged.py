@@ -829,3 +829,23 @@ def test_page_step_outputs_are_ordinary_tensors(cuda_device):
     assert pos.tolist() == [5] * 7
     assert kv.tolist() == [6, 22] and cu.tolist() == [0, 3, 5] and count.tolist() == [1]
     assert torch.cat([kv, cu]).tolist() == [6, 22, 0, 3, 5]
+
+
+def test_default_status_word_is_not_part_of_a_recording(cuda_device, monkeypatch):
+    """The default status word is made by the first eager call, whatever status that call was
+    given: one made while recording would be zeroed by every replay, with what others had
+    reported in it."""
+    monkeypatch.setattr(K, "_STATUS_WORDS", {})
+    monkeypatch.setattr(K, "WORKSPACES", K._Workspaces())
+    c = _Case(cuda_device, [70, 9], [3, 2], 8, 2, 16)
+    c.run(status=torch.zeros(1, dtype=torch.int32, device=cuda_device))
+    out = torch.zeros_like(c.q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(out=out)
+    word = K.attention_status(cuda_device)
+    word.fill_(K.STATUS_PAGES)
+    graph.replay()
+    torch.cuda.synchronize()
+    c.check(out)
+    assert int(word.item()) == K.STATUS_PAGES
