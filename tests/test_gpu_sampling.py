@@ -202,6 +202,33 @@ def test_sample_does_not_depend_on_the_batch_or_strides(cuda_device):
         assert torch.equal(one[0], tok[r:r + 1]) and torch.equal(one[1], logp[r:r + 1])
 
 
+@pytest.mark.parametrize("rows", [7, 40, 100, 300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_full_vocabulary_at_every_launch_shape(cuda_device, rows, dtype):
+    """A batch's size decides how many CTAs share a row (8, 4, 2, 1, or what keeps the rows in
+    flight in L2): every row's token and log-probability are those of the row alone, whatever its
+    rules, and the first rows' those of the definition."""
+    g = torch.Generator(cuda_device).manual_seed(rows)
+    rng = np.random.default_rng(rows)
+    x = torch.empty((rows, gin.V_QWEN3), device=cuda_device).normal_(0, 3, generator=g)
+    x[::3] *= 0.2
+    x[1::7, ::2] = float("nan")
+    x[2::7, 1000:150000] = -math.inf
+    x = x.to(dtype)
+    u = [float(np.float32(v)) for v in rng.random(rows)]
+    temp, k, p, mp = _rules(rng, rows)
+    k = [0 if r % 2 else v for r, v in enumerate(k)]  # half of the rows: top-p alone
+    to = lambda v, dt=torch.float32: torch.tensor(v, dtype=dt, device=cuda_device)  # noqa: E731
+    args = (to(u), to(temp), to(k, torch.int32), to(p), to(mp))
+    tok, logp = K.sample(x, *args)
+    alone = [K.sample(x[r:r + 1], *(a[r:r + 1] for a in args)) for r in range(rows)]
+    assert torch.equal(tok, torch.cat([t for t, _ in alone]))
+    assert torch.equal(logp, torch.cat([v for _, v in alone]))
+    n = 4
+    first = _check(cuda_device, x[:n], u[:n], temp[:n], k[:n], p[:n], mp[:n])
+    assert torch.equal(first[0], tok[:n]) and torch.equal(first[1], logp[:n])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [9, 9001, 40960])
 def test_sample_several_draws_from_one_row(cuda_device, dtype, V):
