@@ -15,6 +15,12 @@
 //      than 2^8 (rescaling O and l), the same decision in every warp
 //   3. write P = 2^(S - m) as bf16 to shared memory; l adds the unrounded values
 //   4. take 32 dims each: O += P V over all 64 keys
+// The matrix instruction takes P as bf16, good to 2^-9.  Units of at most 8 rows (a token of a group
+// of 8 heads) leave half of its 16 rows free: there the other rows hold what the rounding left,
+// P - bf16(P), and the two products are added at the end, so P is good to 2^-17 and the error is
+// that of the output's own rounding (relative 2-norm 1.7e-3; 2.2e-3 with P rounded).  Units of more
+// rows would need instructions of their own for that: 64 x 8 tokens of 9000 keys, 32 rows, 434 to
+// 530 us; there P stays rounded.
 // so K and V leave shared memory once, whether there are 16 rows or 32.  V rows past the request's
 // length may hold anything; their fragments are replaced by zeros in registers.
 // Measured, one token for each of 64 requests of 1k to 32k keys, 32 query heads over 8 (2.38 GB
@@ -141,6 +147,7 @@ __device__ __forceinline__ void merge_rows(const Params& p, const Item& it, int 
 
 // kM: tiles of 16 query rows.  Shared memory: Q (two buffers), P, the ring, maxima / sums, the
 // cost prefix.
+constexpr int unit_rows(int m, bool two_parts) { return two_parts ? 8 : 16 * m; }
 template <int kM>
 struct Layout {
   static constexpr int kRows = 16 * kM;
@@ -154,12 +161,16 @@ struct Layout {
   }
 };
 
-template <int kM>
+// kTwoParts: the unit has at most 8 rows; rows 8 to 15 of its tile hold the second part of P.
+template <int kM, bool kTwoParts>
 __global__ void __launch_bounds__(kShortThreads, 2)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p,
                     const int bufs) {
   using L = Layout<kM>;
+  static_assert(!kTwoParts || kM == 1, "one tile");
+  constexpr int kH = kTwoParts ? 1 : 2;  // rows of a lane in a tile: g, and 8 on
+  constexpr int kUnit = unit_rows(kM, kTwoParts);
   extern __shared__ unsigned char smem_raw[];
   __shared__ ShortBars bars;
   __shared__ long long s_warp[kConsumers + 1];
@@ -172,7 +183,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float* s_max = reinterpret_cast<float*>(smem + L::kRing + bufs * kBufBytes);  // [row][warp]
   long long* s_first = reinterpret_cast<long long*>(s_max + L::kRows * 4);
-  const int unit_tok = L::kRows / p.group;  // tokens a unit has room for
+  const int unit_tok = kUnit / p.group;  // tokens a unit has room for
 
   if (tid == kConsumers * 32) {
     tc::tma_prefetch_desc(&tm_q);
@@ -294,12 +305,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool works = ok;  // the same in all four warps
     const int t0 = it.t0, nt = it.nt, len = it.len;
     const int rows = it.n_tok * p.group;
-    float o[kM][4][4], m[kM][2], l[kM][2];
-    int lim[kM][2];  // keys that the row sees
+    float o[kM][4][4], m[kM][kH], l[kM][kH];
+    int lim[kM][kH];  // keys that the row sees
 #pragma unroll
     for (int a = 0; a < kM; ++a) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kH; ++h) {
         const int r = a * 16 + h * 8 + g;
         lim[a][h] = r < rows ? it.past + r / p.group + 1 : 0x7fffffff;
         m[a][h] = -INFINITY;
@@ -346,7 +357,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
       for (int a = 0; a < kM; ++a)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kH; ++h) {
           const int left = lim[a][h] - kw;
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -367,7 +378,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
       for (int a = 0; a < kM; ++a)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kH; ++h) {
           const float4 w = *reinterpret_cast<const float4*>(&s_max[(a * 16 + h * 8 + g) * 4]);
           const float ms = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * sl2;
           if (ms > m[a][h] + kRescale || (m[a][h] == -INFINITY && ms > -INFINITY)) {
@@ -378,6 +389,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             for (int n = 0; n < 4; ++n) {
               o[a][n][h * 2] *= alpha;
               o[a][n][h * 2 + 1] *= alpha;
+              if (kTwoParts) {
+                o[a][n][2] *= alpha;
+                o[a][n][3] *= alpha;
+              }
             }
           }
           // 3. P
@@ -388,10 +403,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             const float x = tc::ex2_approx(fmaf(s[a][n][h * 2], sl2, nm));
             const float y = tc::ex2_approx(fmaf(s[a][n][h * 2 + 1], sl2, nm));
             l[a][h] += x + y;
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sP + r * 128 +
-                                                         (((warp * 2 + n) ^ (r & 7)) << 4) + t4 * 4),
-                         "r"(tc::pack_bf16x2(x, y))
-                         : "memory");
+            const uint32_t at = sP + r * 128 + (((warp * 2 + n) ^ (r & 7)) << 4) + t4 * 4;
+            const uint32_t xy = tc::pack_bf16x2(x, y);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(xy) : "memory");
+            if (kTwoParts) {
+              const uint32_t rest = tc::pack_bf16x2(x - __uint_as_float(xy << 16),
+                                                    y - __uint_as_float(xy & 0xffff0000u));
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 8 * 128), "r"(rest) : "memory");
+            }
           }
         }
       tc::named_sync(1, kConsumers * 32);
@@ -428,11 +447,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
       release();
     }
+    if (kTwoParts) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        o[0][n][0] += o[0][n][2];
+        o[0][n][1] += o[0][n][3];
+      }
+    }
     // the rows' sums over the warps' keys
 #pragma unroll
     for (int a = 0; a < kM; ++a)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kH; ++h) {
         l[a][h] += __shfl_xor_sync(DDT_FULL_MASK, l[a][h], 1);
         l[a][h] += __shfl_xor_sync(DDT_FULL_MASK, l[a][h], 2);
         if (ok && t4 == 0) s_max[(a * 16 + h * 8 + g) * 4 + warp] = l[a][h];
@@ -443,7 +469,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
     for (int a = 0; a < kM; ++a)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kH; ++h) {
         const int r = a * 16 + h * 8 + g;
         const float4 w = *reinterpret_cast<const float4*>(&s_max[r * 4]);
         const float sum = (w.x + w.y) + (w.z + w.w);
@@ -499,7 +525,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-template <int kM>
+template <int kM, bool kTwoParts>
 int launch_m(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
              const Params& p, cudaStream_t st) {
   using L = Layout<kM>;
@@ -508,11 +534,12 @@ int launch_m(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap
   int bufs = kMaxBufs;
   while (bufs > 2 && L::bytes(bufs, p.n_requests) > kRoom) --bufs;
   const uint32_t smem = L::bytes(bufs, p.n_requests);
-  if (cudaFuncSetAttribute(paged_decode_kernel<kM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(paged_decode_kernel<kM, kTwoParts>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return DDT_ERR_CUDA;
-  return launch_early(paged_decode_kernel<kM>, dim3(kShortCtas), dim3(kShortThreads), smem, st, 0, tm_q,
-                      tm_k, tm_v, p, bufs);
+  return launch_early(paged_decode_kernel<kM, kTwoParts>, dim3(kShortCtas), dim3(kShortThreads), smem,
+                      st, 0, tm_q, tm_k, tm_v, p, bufs);
 }
 
 }  // namespace
@@ -528,16 +555,19 @@ int launch_short(Params& p, const void* q, int64_t q_token_stride, int64_t q_hea
   p.ml_part = p.o_part + kShortPartO / sizeof(float);
   p.arrived = reinterpret_cast<unsigned int*>(p.ml_part + kShortPartMl / sizeof(float));
   p.parts = nullptr;
-  const int m = p.to_new * p.group <= 16 ? 1 : 2;
+  const int rows = p.to_new * p.group, m = rows <= 16 ? 1 : 2;
+  const bool two_parts = rows <= unit_rows(1, true);
   CUtensorMap tm_q;
   const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(q_heads),
                               static_cast<cuuint64_t>(p.n_tokens)};
   const int64_t strides[2] = {q_head_stride, q_token_stride};
   const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group),
-                             static_cast<cuuint32_t>(16 * m / p.group)};
+                             static_cast<cuuint32_t>(unit_rows(m, two_parts) / p.group)};
   const int rc = make_map(&tm_q, q, 3, dims, strides, box);
   if (rc) return rc;
-  return m == 1 ? launch_m<1>(tm_q, tm_k, tm_v, p, st) : launch_m<2>(tm_q, tm_k, tm_v, p, st);
+  return two_parts ? launch_m<1, true>(tm_q, tm_k, tm_v, p, st)
+         : m == 1  ? launch_m<1, false>(tm_q, tm_k, tm_v, p, st)
+                   : launch_m<2, false>(tm_q, tm_k, tm_v, p, st);
 }
 
 }  // namespace paged_attn

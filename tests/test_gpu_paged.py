@@ -390,6 +390,31 @@ def test_paged_attention_sharp_and_flat_scores(cuda_device, name, qscale, scale)
     c.check(out, scale=scale)
 
 
+@pytest.mark.parametrize("hq,hkv,new", [(8, 8, 1), (8, 8, 8), (6, 2, 2), (16, 8, 4), (32, 8, 2),
+                                        (10, 2, 1), (16, 2, 1)])
+def test_paged_attention_weights_of_few_rows(cuda_device, hq, hkv, new):
+    """Up to 8 query rows per (request, KV head) take the softmax weights as two bf16 parts: the
+    first is off by at most 2^-8 of the weight (half a bf16 step), the second by 2^-8 of that.  So an
+    element is off by half a bf16 step of itself, 2^-16 of sum p |v|, and 2^-11 of it for the scores'
+    fp32 sums: 128 products of at most 12 in all, 2^-23 each, in numerator and sum.  Few keys,
+    where the roundings of the weights do not average out, up to many."""
+    rng = np.random.default_rng(hq)
+    lens = [int(n) for n in rng.integers(new, 12, 60)] + [70, 300, 5000]
+    c = _Case(cuda_device, lens, [new] * len(lens), hq, hkv, 16, seed=hq + new)
+    out = c.run()
+    g = hq // hkv
+    for r, n in enumerate(lens):
+        q = c.q64[c.cu[r]:c.cu[r + 1]].view(new, hkv, g, D)
+        s = torch.einsum("ihgd,jhd->hgij", q, c.keys[r]) * D ** -0.5
+        i, j = torch.arange(new, device=s.device)[:, None], torch.arange(n, device=s.device)
+        p = s.masked_fill(j > n - new + i, -math.inf).softmax(-1)
+        ref, mag = (torch.einsum("hgij,jhd->ihgd", p, v).reshape(new, hq, D)
+                    for v in (c.values[r], c.values[r].abs()))
+        tol = ref.abs() * 2.0 ** -8 + mag * (2.0 ** -16 + 2.0 ** -11)
+        err = (out[c.cu[r]:c.cu[r + 1]].double() - ref).abs()
+        assert bool((err <= tol).all()), (r, n, int((err > tol).sum()), float((err / tol).max()))
+
+
 def test_paged_attention_is_repeatable(cuda_device):
     lens, news, hq, hkv, page = ATTN["chunk_among_decodes"]
     c = _Case(cuda_device, lens, news, hq, hkv, page, seed=3)
