@@ -25,7 +25,7 @@
 // length may hold anything; their fragments are replaced by zeros in registers.
 // Measured, one token for each of 64 requests of 1k to 32k keys, 32 query heads over 8 (2.38 GB
 // of K and V): 362 us, 6.57 TB/s, the measured copy rate, with 1.003 times the bytes read from
-// HBM.  One request of 1000 keys takes 9.7 us, two thirds of it dependent reads (lengths, page
+// HBM.  One request of 1000 keys takes 9.1 to 9.7 us, two thirds of it dependent reads (lengths, page
 // ids, K, the parts).
 // Units are cut over the CTAs as in paged_sched.cuh; the CTA that brings a cut unit's last part
 // merges all of them, in the order of the CTAs, so the result does not depend on which it is, and
