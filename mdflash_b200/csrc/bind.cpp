@@ -222,7 +222,8 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   const auto call = [&](auto entry, const char* name, auto... wait) {
     check(entry(ptr(q), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages), pool.pages, pool.page,
                 pool.page_stride, pool.head_stride, pool.row_stride, ptr<int32_t>(block_table),
-                table.first, table.second, ptr<int32_t>(cu_new), ptr<int32_t>(kv_lens), R, T, max_new, hq, pool.heads, d,
+                table.first, table.second, ptr<int32_t>(cu_new), ptr<int32_t>(kv_lens), R, T, max_new,
+                hq, pool.heads, d,
                 static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(d))), ptr(o),
                 o.stride(0), o.stride(1), ptr(workspace), workspace.numel(), ptr<int32_t>(status),
                 wait..., stream_of(idx)),
